@@ -52,6 +52,11 @@ SIGNATURES = {
     ),
     "rpa_mla_workspace_bytes": (_c_sz, [_c_int] * 8),
     "rpa_mla_page_scatter": (_c_int, [_c_vp] * 8 + [_c_int] * 9),
+    "rpa_rope_page_scatter_ragged": (_c_int, [_c_vp] * 13 + [_c_int] * 13 + [_c_i64] * 3 + [_c_int] * 2),
+    "rpa_rope_unified_page_scatter": (_c_int, [_c_vp] * 13 + [_c_int] * 11 + [_c_i64] * 3 + [_c_int] * 2),
+    "rpa_rope_mla_page_scatter": (_c_int, [_c_vp] * 12 + [_c_int] * 11 + [_c_i64] * 2 + [_c_int] * 2),
+    "rpa_decay_linear_attention": (_c_int, [_c_vp] * 13 + [_c_sz] + [_c_int] * 7 + [_c_i64] * 3 + [_c_int, _c_f32]),
+    "rpa_decay_attention_workspace_bytes": (_c_sz, [_c_int] * 7),
 }
 
 

@@ -30,6 +30,8 @@ SOURCES = [
     "rpa_widen.hip",
     "rpa_attn_merge.hip",
     "rpa_mla.hip",
+    "rpa_rope.hip",
+    "rpa_decay.hip",
 ]
 # measurement kernels and result-changing test knobs: compiled into the test / benchmark build only (-DRPA_PROBES)
 PROBE_SOURCES = ["rpa_probe.hip"]

@@ -9,7 +9,9 @@
 
 #include "../../include/rpa_hip_probe.h"
 #include "rpa_common.h"
+#include "rpa_decay.h"
 #include "rpa_mla.h"
+#include "rpa_rope.h"
 
 namespace rpa {
 int launch_scatter_slices(hipStream_t, const void*, const int32_t*, const int32_t*, void*, int, int, int64_t, int,
@@ -797,6 +799,171 @@ int rpa_mla_ragged_paged_attention(rpa_stream_t stream, const void* queries_nope
     if (err) return hip_fail(err, "MLA fp32 kernel launch");
   }
   return hip_fail(rpa::launch_mla_merge(s, p), "MLA merge kernel launch");
+}
+
+// What the three append-with-rotation entry points share: sizes, the rotation's table and the ragged metadata.
+static int rope_fill(const char* who, rpa::RopeParams& p, const void* query, const void* key, const void* query_out,
+                     const float* cos_sin, const int32_t* positions, const int32_t* context_lens, const int32_t* block_tables,
+                     const int32_t* query_start_loc, const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int Hkv,
+                     int D, int rope_dim, int table_rows, int neox_style, int64_t query_stride, int64_t key_stride, int src_dtype, int kv_dtype) {
+  if (T < 0 || S <= 0 || M <= 0 || P <= 0 || page_size <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || rope_dim <= 0 || table_rows <= 0)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: bad size (T=%d S=%d M=%d P=%d page_size=%d Hq=%d Hkv=%d D=%d rope_dim=%d table_rows=%d)", who,
+                T, S, M, P, page_size, Hq, Hkv, D, rope_dim, table_rows);
+  if (rope_dim % 2 != 0 || rope_dim > D) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: rope_dim %d (want even, at most the head size %d)", who, rope_dim, D);
+  if (D % 2 != 0) return fail(RPA_ERR_UNSUPPORTED, "%s: head size %d is odd", who, D);
+  if (neox_style != 0 && neox_style != 1) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: neox_style %d (want 0 or 1)", who, neox_style);
+  if (src_dtype != RPA_F32 && src_dtype != RPA_BF16 && src_dtype != RPA_F16)
+    return fail(RPA_ERR_UNSUPPORTED, "%s: source dtype %d (want f32, bf16 or f16)", who, src_dtype);
+  if (kv_dtype < RPA_F32 || kv_dtype > RPA_F16) return fail(RPA_ERR_UNSUPPORTED, "%s: page dtype %d", who, kv_dtype);
+  if ((int64_t)M * page_size > INT32_MAX) return fail(RPA_ERR_UNSUPPORTED, "%s: block-table rows of %d pages of %d tokens address more than 2^31 - 1 positions", who, M, page_size);
+  if ((int64_t)S * 2 + (int64_t)T / page_size > INT32_MAX / 2) return fail(RPA_ERR_UNSUPPORTED, "%s: %d sequences are too many", who, S);
+  if (T == 0) return RPA_OK;
+  if (!query || !key || !query_out || !cos_sin || !context_lens || !block_tables || !query_start_loc)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  const int e = rpa::elem_bytes(src_dtype);
+  if ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)query_out)) % e || ((uintptr_t)cos_sin & 3))
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: an operand is not aligned to its elements", who);
+  memset(&p, 0, sizeof(p));
+  p.q = query; p.k = key; p.q_out = (void*)query_out; p.cos_sin = cos_sin; p.positions = positions;
+  p.context_lens = context_lens; p.block_tables = block_tables; p.qsl = query_start_loc; p.num_seqs = num_seqs;
+  p.T = T; p.S = S; p.M = M; p.P = P; p.page_size = page_size; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.rope = rope_dim;
+  p.table_rows = table_rows; p.neox = neox_style; p.q_stride = query_stride; p.k_stride = key_stride;
+  p.src_dtype = src_dtype; p.kv_dtype = kv_dtype;
+  p.q_in_place = query == query_out;
+  if (p.q_in_place && query_stride != (int64_t)Hq * D)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: query_out is query, whose rows are not contiguous", who);
+  return RPA_OK;
+}
+
+static int check_strides(const char* who, int64_t query_stride, int64_t q_row, int64_t key_stride, int64_t k_row, int64_t value_stride, int64_t v_row) {
+  if (query_stride < q_row || key_stride < k_row || value_stride < v_row)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: token rows overlap (strides %lld, %lld, %lld; rows %lld, %lld, %lld)", who, (long long)query_stride,
+                (long long)key_stride, (long long)value_stride, (long long)q_row, (long long)k_row, (long long)v_row);
+  return RPA_OK;
+}
+
+int rpa_rope_page_scatter_ragged(rpa_stream_t stream, const void* query, const void* key, const void* value, void* query_out,
+                                 void* kv_pages, float* kv_scales, const float* cos_sin, const int32_t* positions,
+                                 const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                                 const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int Hkv, int D,
+                                 int Dp, int C, int rope_dim, int table_rows, int neox_style, int64_t query_stride,
+                                 int64_t key_stride, int64_t value_stride, int src_dtype, int kv_dtype) {
+  const char* who = "rpa_rope_page_scatter_ragged";
+  rpa::RopeParams p;
+  if (const int rc = rope_fill(who, p, query, key, query_out, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs, T, S, M, P,
+                               page_size, Hq, Hkv, D, rope_dim, table_rows, neox_style, query_stride, key_stride, src_dtype, kv_dtype)) return rc;
+  if (const int rc = check_strides(who, query_stride, (int64_t)Hq * D, key_stride, (int64_t)Hkv * D, value_stride, (int64_t)Hkv * D)) return rc;
+  if (C < 2 * Hkv) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: C=%d combined heads < 2 * Hkv=%d", who, C, Hkv);
+  const int ek = rpa::elem_bytes(kv_dtype);
+  if (const int rc = check_row_width(who, D, Dp, ek)) return rc;
+  if (Dp % 2 != 0) return fail(RPA_ERR_UNSUPPORTED, "%s: stored head width %d is odd", who, Dp);
+  const bool eight = kv_dtype == RPA_FP8_E4M3 || kv_dtype == RPA_INT8;
+  if (kv_dtype == RPA_INT8 && !kv_scales) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: int8 KV pages need kv_scales", who);
+  if (kv_scales && !eight) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: kv_scales with pages that are not 8-bit", who);
+  if (T == 0) return RPA_OK;
+  if (!value || !kv_pages || !num_seqs) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if ((uintptr_t)value % rpa::elem_bytes(src_dtype) || ((uintptr_t)kv_pages & 3) || ((uintptr_t)kv_scales & 3))
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: value must be aligned to its elements, kv_pages and kv_scales to 4 bytes", who);
+  p.v = value; p.v_stride = value_stride; p.scales = kv_scales; p.Dp = Dp; p.C = C;
+  p.token_stride = (int64_t)C * Dp * ek;
+  p.page_stride = p.token_stride * page_size;
+  p.head_stride = 2 * (int64_t)Dp * ek;
+  p.k_pages = (char*)kv_pages;
+  p.v_pages = (char*)kv_pages + (int64_t)Dp * ek;
+  hipStream_t s = (hipStream_t)stream;
+  return hip_fail(kv_scales ? rpa::launch_rope_append_quant(s, p) : rpa::launch_rope_append(s, p), "rpa_rope_page_scatter_ragged launch");
+}
+
+int rpa_rope_unified_page_scatter(rpa_stream_t stream, const void* query, const void* key, const void* value, void* query_out,
+                                  void* key_cache, void* value_cache, const float* cos_sin, const int32_t* positions,
+                                  const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                                  const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int Hkv, int D,
+                                  int rope_dim, int table_rows, int neox_style, int64_t query_stride, int64_t key_stride,
+                                  int64_t value_stride, int src_dtype, int kv_dtype) {
+  const char* who = "rpa_rope_unified_page_scatter";
+  rpa::RopeParams p;
+  if (const int rc = rope_fill(who, p, query, key, query_out, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs, T, S, M, P,
+                               page_size, Hq, Hkv, D, rope_dim, table_rows, neox_style, query_stride, key_stride, src_dtype, kv_dtype)) return rc;
+  if (const int rc = check_strides(who, query_stride, (int64_t)Hq * D, key_stride, (int64_t)Hkv * D, value_stride, (int64_t)Hkv * D)) return rc;
+  if (kv_dtype == RPA_INT8) return fail(RPA_ERR_UNSUPPORTED, "%s: int8 pools (want f32, bf16, f16 or fp8-e4m3 without scales)", who);
+  const int ek = rpa::elem_bytes(kv_dtype);
+  if (const int rc = check_row_width(who, D, D, ek)) return rc;
+  if (T == 0) return RPA_OK;
+  if (!value || !key_cache || !value_cache) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if ((uintptr_t)value % rpa::elem_bytes(src_dtype) || ((((uintptr_t)key_cache) | ((uintptr_t)value_cache)) & 3))
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: value must be aligned to its elements, the pools to 4 bytes", who);
+  p.v = value; p.v_stride = value_stride; p.Dp = D; p.C = 2 * Hkv;
+  p.head_stride = (int64_t)D * ek;
+  p.token_stride = p.head_stride * Hkv;
+  p.page_stride = p.token_stride * page_size;
+  p.k_pages = (char*)key_cache;
+  p.v_pages = (char*)value_cache;
+  return hip_fail(rpa::launch_rope_append((hipStream_t)stream, p), "rpa_rope_unified_page_scatter launch");
+}
+
+int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const void* keys_values, const void* keys_pe,
+                              void* queries_pe_out, void* kv_pages, const float* cos_sin, const int32_t* positions,
+                              const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                              const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int kv_lora_rank,
+                              int qk_rope_head_dim, int row_elems, int table_rows, int neox_style, int64_t query_stride,
+                              int64_t key_stride, int src_dtype, int kv_dtype) {
+  const char* who = "rpa_rope_mla_page_scatter";
+  rpa::MlaParams m;  // the latent pages' own checks
+  if (const int rc = mla_fill(who, m, keys_values, keys_pe, kv_pages, context_lens, block_tables, query_start_loc, num_seqs, T, S, M, P, page_size,
+                              kv_lora_rank, qk_rope_head_dim, row_elems, kv_dtype)) return rc;
+  rpa::RopeParams p;
+  if (const int rc = rope_fill(who, p, queries_pe, keys_pe, queries_pe_out, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs,
+                               T, S, M, P, page_size, Hq, 1, qk_rope_head_dim, qk_rope_head_dim, table_rows, neox_style, query_stride, key_stride,
+                               src_dtype, kv_dtype)) return rc;
+  if (const int rc = check_strides(who, query_stride, (int64_t)Hq * qk_rope_head_dim, key_stride, qk_rope_head_dim, 0, 0)) return rc;
+  if (row_elems % 4 != 0) return fail(RPA_ERR_UNSUPPORTED, "%s: row_elems %d is not a multiple of 4", who, row_elems);
+  if (T == 0) return RPA_OK;
+  if (!keys_values || !kv_pages || !num_seqs) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if ((((uintptr_t)keys_values) | ((uintptr_t)kv_pages)) & 3) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: keys_values and kv_pages must be 4-byte aligned", who);
+  p.latent = keys_values; p.lkv = kv_lora_rank; p.rope_off = m.rope_off; p.row_elems = row_elems;
+  p.Dp = qk_rope_head_dim;
+  p.token_stride = m.token_stride; p.page_stride = m.page_stride;
+  p.k_pages = (char*)kv_pages;
+  return hip_fail(rpa::launch_rope_latent((hipStream_t)stream, p), "rpa_rope_mla_page_scatter launch");
+}
+
+size_t rpa_decay_attention_workspace_bytes(int T, int S, int Hq, int Hkv, int Dk, int Dv, int dtype) {
+  (void)T; (void)S; (void)Hq; (void)Hkv; (void)Dk; (void)Dv; (void)dtype;
+  return 0;
+}
+
+int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const void* key, const void* value, const float* log_decay,
+                               float* state, const int32_t* state_indices, const int32_t* state_out_indices,
+                               const int32_t* context_lens, const int32_t* query_start_loc, const int32_t* num_seqs, void* out,
+                               void* workspace, size_t workspace_bytes, int T, int S, int num_slots, int Hq, int Hkv, int Dk,
+                               int Dv, int64_t query_stride, int64_t key_stride, int64_t value_stride, int dtype, float scale) {
+  const char* who = "rpa_decay_linear_attention";
+  if (T < 0 || S <= 0 || num_slots <= 0 || Hq <= 0 || Hkv <= 0 || Dk <= 0 || Dv <= 0)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: bad size (T=%d S=%d num_slots=%d Hq=%d Hkv=%d Dk=%d Dv=%d)", who, T, S, num_slots, Hq, Hkv, Dk, Dv);
+  if (Hq % Hkv != 0) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: Hq=%d is not a multiple of Hkv=%d", who, Hq, Hkv);
+  if (Dk % 4 != 0 || Dv % 4 != 0 || Dk > 256 || Dv > 256)
+    return fail(RPA_ERR_UNSUPPORTED, "%s: key size %d / value size %d (want multiples of 4, at most 256)", who, Dk, Dv);
+  if (dtype != RPA_F32 && dtype != RPA_BF16 && dtype != RPA_F16) return fail(RPA_ERR_UNSUPPORTED, "%s: dtype %d (want f32, bf16 or f16)", who, dtype);
+  if (S > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: %d sequences (at most 65535)", who, S);
+  if (!std::isfinite(scale)) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: scale is not finite", who);
+  if (const int rc = check_strides(who, query_stride, (int64_t)Hq * Dk, key_stride, (int64_t)Hkv * Dk, value_stride, (int64_t)Hkv * Dv)) return rc;
+  if (T == 0) return RPA_OK;
+  if (!query || !key || !value || !log_decay || !state || !state_indices || !query_start_loc || !num_seqs || !out)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  const int e = rpa::elem_bytes(dtype);
+  if ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)value)) % e || (((uintptr_t)out) | ((uintptr_t)state)) & 15)
+    return fail(RPA_ERR_INVALID_ARGUMENT, "%s: query, key and value must be aligned to their elements, out and state to 16 bytes", who);
+  const size_t need = rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(RPA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
+  rpa::DecayParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = query; p.k = key; p.v = value; p.log_decay = log_decay; p.state = state;
+  p.slot_in = state_indices; p.slot_out = state_out_indices ? state_out_indices : state_indices;
+  p.context_lens = context_lens; p.qsl = query_start_loc; p.num_seqs = num_seqs; p.out = out;
+  p.T = T; p.S = S; p.num_slots = num_slots; p.Hq = Hq; p.Hkv = Hkv; p.group = Hq / Hkv; p.Dk = Dk; p.Dv = Dv;
+  p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.dtype = dtype; p.scale = scale;
+  return hip_fail(rpa::launch_decay_recurrent((hipStream_t)stream, p), "rpa_decay_linear_attention launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,115 @@
+// Linear attention with one decay per KV head, recurrent form:
+//     S <- l S + k_t v_t^T,   o_t = scale * q_t S.
+// For few tokens the state is the traffic: 4 Dk Dv bytes read and as many written per head and sequence against 2 (Dk + Dv)
+// elements of q, k, v, o per token, so the kernel is bound by HBM.  A workgroup owns 4 CG columns of one head's state in
+// registers: thread (r, c) holds rows r, r + RG, ... of four columns, read in 16-byte loads that are all in flight before the
+// first is used.
+#include "rpa_decay.h"
+
+namespace rpa {
+
+namespace {
+
+template <int DT, int CG, int NR>  // CG groups of four columns, NR rows per thread
+__global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayParams p) {
+  constexpr int RG = 256 / CG;
+  constexpr int MAXD = 256;
+  __shared__ float sk[MAXD], sq[MAXD], sv[4 * CG];
+  __shared__ float4 part[4][CG];
+  const int i = blockIdx.y, slices = (p.Dv + 4 * CG - 1) / (4 * CG);
+  const int h = blockIdx.x / slices, c0 = (blockIdx.x - h * slices) * 4 * CG;
+  const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
+  const DecaySeq s = decay_seq(p, i);
+  if (s.q_len <= 0) return;
+  const int col = c0 + 4 * cg;
+  const bool in_cols = col < p.Dv;
+  const int64_t head = (int64_t)p.Dk * p.Dv, at = (int64_t)h * head + col;
+  float4 S[NR];
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const int r = rg + j * RG;
+    S[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s.in >= 0 && in_cols && r < p.Dk) S[j] = *(const float4*)(p.state + (int64_t)s.in * p.Hkv * head + at + (int64_t)r * p.Dv);
+  }
+  const float2 l = decay_power(p.log_decay[h], 1);
+  for (int n = 0; n < s.q_len; ++n) {
+    const int64_t t = s.q0 + n;
+    for (int d = tid; d < p.Dk; d += 256) sk[d] = load_elem<DT>(p.k, t * p.k_stride + h * p.Dk + d);
+    for (int d = tid; d < 4 * CG; d += 256) sv[d] = c0 + d < p.Dv ? load_elem<DT>(p.v, t * p.v_stride + h * p.Dv + c0 + d) : 0.f;
+    for (int g = 0; g < p.group; ++g) {
+      const int hq = h * p.group + g;
+      for (int d = tid; d < p.Dk; d += 256) sq[d] = load_elem<DT>(p.q, t * p.q_stride + hq * p.Dk + d);
+      __syncthreads();
+      if (g == 0) {
+        const float4 v = *(const float4*)&sv[4 * cg];
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+          const int r = rg + j * RG;
+          const float k = r < p.Dk ? sk[r] : 0.f;
+          S[j].x = fmaf(S[j].x, l.y, fmaf(S[j].x, l.x, k * v.x));
+          S[j].y = fmaf(S[j].y, l.y, fmaf(S[j].y, l.x, k * v.y));
+          S[j].z = fmaf(S[j].z, l.y, fmaf(S[j].z, l.x, k * v.z));
+          S[j].w = fmaf(S[j].w, l.y, fmaf(S[j].w, l.x, k * v.w));
+        }
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const int r = rg + j * RG;
+        const float q = r < p.Dk ? sq[r] : 0.f;
+        o.x = fmaf(q, S[j].x, o.x); o.y = fmaf(q, S[j].y, o.y); o.z = fmaf(q, S[j].z, o.z); o.w = fmaf(q, S[j].w, o.w);
+      }
+#pragma unroll
+      for (int m = 32; m >= CG; m >>= 1) {
+        o.x += __shfl_xor(o.x, m); o.y += __shfl_xor(o.y, m); o.z += __shfl_xor(o.z, m); o.w += __shfl_xor(o.w, m);
+      }
+      if ((tid & 63) < CG) part[tid >> 6][cg] = o;
+      __syncthreads();
+      if (tid < 4 * CG && c0 + tid < p.Dv) {
+        const float* f = (const float*)part;
+        const float r = (f[tid] + f[4 * CG + tid]) + (f[8 * CG + tid] + f[12 * CG + tid]);
+        store_out<DT>(p.out, (t * p.Hq + hq) * p.Dv + c0 + tid, r * p.scale);
+      }
+    }
+  }
+  if (s.out < 0 || !in_cols) return;
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const int r = rg + j * RG;
+    if (r < p.Dk) *(float4*)(p.state + (int64_t)s.out * p.Hkv * head + at + (int64_t)r * p.Dv) = S[j];
+  }
+}
+
+// Rows of tokens that belong to no sequence.
+__global__ __launch_bounds__(256) void decay_pad_kernel(DecayParams p, int row_bytes) {
+  const int t = blockIdx.x, n = decay_live_rows(p);
+  if (n > 0 && t >= p.qsl[0] && t < p.qsl[n]) return;
+  uint32_t* row = (uint32_t*)((char*)p.out + (int64_t)t * row_bytes);
+  for (int k = threadIdx.x; k < row_bytes / 4; k += 256) row[k] = 0u;
+}
+
+template <int DT, int CG>
+int launch_cols(hipStream_t stream, const DecayParams& p) {
+  constexpr int RG = 256 / CG;
+  const int slices = (p.Dv + 4 * CG - 1) / (4 * CG);
+  const dim3 grid(p.Hkv * slices, p.S), block(256);
+  const int need = (p.Dk + RG - 1) / RG;
+  if (need <= 64 / RG) hipLaunchKernelGGL((decay_recurrent_kernel<DT, CG, 64 / RG>), grid, block, 0, stream, p);
+  else if (need <= 128 / RG) hipLaunchKernelGGL((decay_recurrent_kernel<DT, CG, 128 / RG>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((decay_recurrent_kernel<DT, CG, 256 / RG>), grid, block, 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_decay_recurrent(hipStream_t stream, const DecayParams& p) {
+  hipLaunchKernelGGL(decay_pad_kernel, dim3(p.T), dim3(256), 0, stream, p, p.Hq * p.Dv * elem_bytes(p.dtype));
+  switch (p.dtype) {
+    case RPA_F32: return launch_cols<RPA_F32, 8>(stream, p);
+    case RPA_BF16: return launch_cols<RPA_BF16, 8>(stream, p);
+    case RPA_F16: return launch_cols<RPA_F16, 8>(stream, p);
+    default: return (int)hipErrorInvalidValue;
+  }
+}
+
+}  // namespace rpa

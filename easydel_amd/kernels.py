@@ -426,3 +426,248 @@ def mla_ragged_paged_attention(queries_nope, queries_pe, keys_values, keys_pe, k
             _i32(distribution, "distribution"), _dev(out, "out"), ws.data_ptr(), ws.numel(),
             T, S, M, P, pg, Hq, lkv, rope, row, qd, kd, scale, window, cap, aux_ptr))
     return out, kv_pages
+
+
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device) -> tuple[int, int]:
+    """(pointer, elements between token rows) of a ``[T, heads, dim]`` or ``[T, dim]`` operand whose token rows are
+    contiguous and may lie apart, as views of one projection's output do."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor holding device memory, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}; the ROCm ragged-page kernels need GPU memory (no CPU fallback)")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the query on {device}")
+    row, want = math.prod(shape[1:]), 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and stride != want:
+            raise ValueError(f"{name}: the elements of a token row must be contiguous, got strides {t.stride()}")
+        want *= size
+    return t.data_ptr(), row if t.shape[0] <= 1 else t.stride(0)
+
+
+def _on(t: torch.Tensor, name: str, dtype: torch.dtype, device) -> int:
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    ptr = _dev(t, name)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the query on {device}")
+    return ptr
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _turned_out(query, query_out, others, name: str):
+    """The tensor the turned queries go to: a new one, the queries themselves, or one that overlaps no operand."""
+    if query_out is None:
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if query_out.shape != query.shape or query_out.dtype != query.dtype or query_out.device != query.device:
+        raise ValueError(f"{name} must be {list(query.shape)} {query.dtype} on {query.device}, got {list(query_out.shape)} "
+                         f"{query_out.dtype} on {query_out.device}")
+    if not query_out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    a, b = _span(query_out)
+    in_place = query_out.data_ptr() == query.data_ptr() and query.is_contiguous()
+    for t in others if in_place else (query, *others):
+        c, d = _span(t)
+        if a < d and c < b:
+            raise ValueError(f"{name} overlaps another operand (only the contiguous queries themselves may be given)")
+    return query_out
+
+
+def _table(cos_sin, rope_dim: int | None, dim: int, device) -> tuple[int, int, int]:
+    """(pointer, rotated elements, rows) of a float32 ``[rows, rope_dim]`` table: cosines, then sines."""
+    if cos_sin.ndim != 2:
+        raise ValueError(f"cos_sin must be [positions, rope_dim], got {list(cos_sin.shape)}")
+    rows, width = cos_sin.shape
+    if rows == 0 or width == 0 or width % 2 or width > dim:
+        raise ValueError(f"cos_sin [positions, rope_dim] must hold a row and an even rope_dim of at most {dim}, got {list(cos_sin.shape)}")
+    if rope_dim is not None and width != rope_dim:
+        raise ValueError(f"cos_sin has rows of {width}, the rope part is {rope_dim} wide")
+    return _on(cos_sin, "cos_sin", torch.float32, device), width, rows
+
+
+def _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T: int, device):
+    """(S, M, pointers of context_lens, block_tables, query_start_loc, num_seqs, positions), checked against each other."""
+    S = context_lens.shape[0]
+    if S == 0 or block_tables.numel() == 0 or block_tables.numel() % S:
+        raise ValueError("block_tables size is not a multiple of the number of sequence rows")
+    if query_start_loc.numel() != S + 1:
+        raise ValueError(f"query_start_loc must hold {S + 1} entries, got {query_start_loc.numel()}")
+    if num_seqs is not None and num_seqs.numel() < 1:
+        raise ValueError("num_seqs is empty")
+    if positions is not None and tuple(positions.shape) != (T,):
+        raise ValueError(f"positions must be [{T}], got {list(positions.shape)}")
+    i32 = torch.int32
+    return (S, block_tables.numel() // S, _on(context_lens, "context_lens", i32, device), _on(block_tables, "block_tables", i32, device),
+            _on(query_start_loc, "query_start_loc", i32, device), None if num_seqs is None else _on(num_seqs, "num_seqs", i32, device),
+            None if positions is None else _on(positions, "positions", i32, device))
+
+
+def _rope_operands(query, key, value):
+    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
+        raise ValueError(f"query [T, Hq, D] and key, value [T, Hkv, D] expected, got {list(query.shape)}, {list(key.shape)}, {list(value.shape)}")
+    T, Hq, D = query.shape
+    Hkv = key.shape[1]
+    dev, dt = query.device, query.dtype
+    if dt not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"query must be float32, bfloat16 or float16, got {dt}")
+    return (T, Hq, Hkv, D, _rows(query, "query", (T, Hq, D), dt, dev), _rows(key, "key", (T, Hkv, D), dt, dev),
+            _rows(value, "value", (T, Hkv, D), dt, dev))
+
+
+def rope_page_scatter_ragged(query, key, value, kv_pages, cos_sin, context_lens, block_tables, query_start_loc, num_seqs, *,
+                             kv_scales=None, positions=None, is_neox_style: bool = True, query_out=None):
+    """Rotary position embedding and page write in one launch: ``query [T, Hq, D]`` and ``key [T, Hkv, D]`` turn by the
+    angles of their positions, the keys and ``value`` go to the pages as :func:`page_scatter_ragged` places them (scaled
+    8-bit pages: coded from the turned float32 keys as :func:`page_scatter_ragged_quantised` codes them, with the scale
+    ``amax * (1 / qmax)`` in the place of ``amax / qmax``).
+
+    ``cos_sin [rows, rope_dim]`` float32 holds the cosines, then the sines, of a position's angles; a token's row is its
+    cache position, or ``positions [T]``, clamped into the table.  The first ``rope_dim`` elements of a head turn, in
+    pairs ``(d, d + rope_dim / 2)`` (``is_neox_style``) or ``(2 d, 2 d + 1)``.  The token rows of query, key and value may lie
+    apart (views of one projection).  Returns ``(turned query, kv_pages)``, with scales ``(..., kv_scales)``; rows of
+    padded tokens of the turned query are zeros (``query_out=query`` turns it in place and leaves them)."""
+    lib = _lib.load()
+    T, Hq, Hkv, D, (q, qs), (k, ks), (v, vs) = _rope_operands(query, key, value)
+    P, pg, C, Dp = page_geometry(kv_pages, D)
+    kd = dtype_tag(kv_pages.dtype)
+    if kv_scales is not None and (kv_scales.dtype != torch.float32 or kv_scales.numel() != P * C):
+        raise ValueError(f"kv_scales must be float32 [P={P}, C={C}]")
+    dev = query.device
+    table, rope, rows = _table(cos_sin, None, D, dev)
+    S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
+    out = _turned_out(query, query_out, (key, value), "query_out")
+    pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
+    scales = None if kv_scales is None else _on(kv_scales, "kv_scales", torch.float32, dev)
+    if T > 0:
+        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
+            _lib.check(lib.rpa_rope_page_scatter_ragged(
+                _stream(query), q, k, v, out.data_ptr(), pages, scales, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, Dp, C,
+                rope, rows, int(bool(is_neox_style)), qs, ks, vs, dtype_tag(query.dtype), kd))
+    return (out, kv_pages) if kv_scales is None else (out, kv_pages, kv_scales)
+
+
+def rope_unified_page_scatter(query, key, value, key_cache, value_cache, cos_sin, context_lens, block_tables, query_start_loc,
+                              num_seqs=None, *, positions=None, is_neox_style: bool = True, query_out=None):
+    """:func:`rope_page_scatter_ragged` into separate K and V pools ``[P, page_size, Hkv, D]`` (without scales).  Without
+    ``num_seqs`` every row of ``context_lens`` is live.  Returns ``(turned query, key_cache, value_cache)``."""
+    lib = _lib.load()
+    T, Hq, Hkv, D, (q, qs), (k, ks), (v, vs) = _rope_operands(query, key, value)
+    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+        raise ValueError(f"key_cache {tuple(key_cache.shape)} {key_cache.dtype} and value_cache "
+                         f"{tuple(value_cache.shape)} {value_cache.dtype} must match")
+    if key_cache.ndim != 4 or tuple(key_cache.shape[2:]) != (Hkv, D):
+        raise ValueError(f"key_cache must be [P, page_size, {Hkv}, {D}], got {tuple(key_cache.shape)}")
+    P, pg = key_cache.shape[:2]
+    kd, dev = dtype_tag(key_cache.dtype), query.device
+    table, rope, rows = _table(cos_sin, None, D, dev)
+    S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
+    out = _turned_out(query, query_out, (key, value), "query_out")
+    kc, vc = _on(key_cache, "key_cache", key_cache.dtype, dev), _on(value_cache, "value_cache", key_cache.dtype, dev)
+    if T > 0:
+        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
+            _lib.check(lib.rpa_rope_unified_page_scatter(
+                _stream(query), q, k, v, out.data_ptr(), kc, vc, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, rope, rows,
+                int(bool(is_neox_style)), qs, ks, vs, dtype_tag(query.dtype), kd))
+    return out, key_cache, value_cache
+
+
+def rope_mla_page_scatter(queries_pe, keys_values, keys_pe, kv_pages, cos_sin, context_lens, block_tables, query_start_loc, num_seqs, *,
+                          positions=None, is_neox_style: bool = True, query_out=None):
+    """The rotation of multi-latent attention and its page write in one launch: ``queries_pe [T, Hq, rope]`` turn,
+    ``keys_pe [T, rope]`` turn into the latent rows, ``keys_values [T, kv_lora_rank]`` (already in the pages' element type) are
+    copied beside them as :func:`mla_page_scatter` places them.  Table, positions, styles and padded rows as for
+    :func:`rope_page_scatter_ragged`, over the whole rope part.  Returns ``(turned queries_pe, kv_pages)``."""
+    lib = _lib.load()
+    if queries_pe.ndim != 3 or keys_pe.ndim != 2 or keys_values.ndim != 2:
+        raise ValueError(f"queries_pe [T, Hq, rope], keys_pe [T, rope] and keys_values [T, kv_lora_rank] expected, got "
+                         f"{list(queries_pe.shape)}, {list(keys_pe.shape)}, {list(keys_values.shape)}")
+    T, Hq, rope = queries_pe.shape
+    dev, dt = queries_pe.device, queries_pe.dtype
+    if dt not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"queries_pe must be float32, bfloat16 or float16, got {dt}")
+    q, qs = _rows(queries_pe, "queries_pe", (T, Hq, rope), dt, dev)
+    k, ks = _rows(keys_pe, "keys_pe", (T, rope), dt, dev)
+    if keys_values.shape[0] != T:
+        raise ValueError(f"keys_values must hold {T} rows, got {keys_values.shape[0]}")
+    lkv = keys_values.shape[1]
+    P, pg, row = mla_row_geometry(kv_pages)
+    kd = dtype_tag(kv_pages.dtype)
+    latent = _on(keys_values, "keys_values", kv_pages.dtype, dev)
+    table, _, rows = _table(cos_sin, rope, rope, dev)
+    S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
+    out = _turned_out(queries_pe, query_out, (keys_pe, keys_values), "query_out")
+    pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
+    if T > 0:
+        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
+            _lib.check(lib.rpa_rope_mla_page_scatter(
+                _stream(queries_pe), q, latent, k, out.data_ptr(), pages, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, lkv, rope, row, rows,
+                int(bool(is_neox_style)), qs, ks, dtype_tag(dt), kd))
+    return out, kv_pages
+
+
+def decay_linear_attention(query, key, value, log_decay, state, state_indices, query_start_loc, num_seqs, *, context_lens=None,
+                           state_out_indices=None, scale: float | None = None, out=None):
+    """Linear attention with one decay per KV head over a ragged batch; the states live in the slots of a pool.
+
+    For the tokens of a sequence in order, ``S <- exp(log_decay[h]) S + k v^T`` and ``out = scale * q S``, with ``query
+    [T, Hq, Dk]``, ``key [T, Hkv, Dk]``, ``value [T, Hkv, Dv]`` of one dtype (float32, bfloat16, float16; token rows may lie
+    apart) and ``state [slots, Hkv, Dk, Dv]`` float32, one state to ``Hq / Hkv`` query heads.  Sequence ``i`` goes on from slot
+    ``state_indices[i]``, or from zero where ``context_lens[i]`` says that it has no tokens before these, and leaves its
+    state in ``state_out_indices[i]`` (default: the same slot).  ``scale`` defaults to ``Dk ** -0.5``.  Returns ``(out [T, Hq,
+    Dv], state)``: the pool updated in place, rows of padded tokens zeros."""
+    lib = _lib.load()
+    if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
+        raise ValueError(f"query [T, Hq, Dk], key [T, Hkv, Dk] and value [T, Hkv, Dv] expected, got {list(query.shape)}, "
+                         f"{list(key.shape)}, {list(value.shape)}")
+    T, Hq, Dk = query.shape
+    Hkv, Dv = key.shape[1], value.shape[2]
+    dev, dt = query.device, query.dtype
+    if dt not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"query must be float32, bfloat16 or float16, got {dt}")
+    q, qs = _rows(query, "query", (T, Hq, Dk), dt, dev)
+    k, ks = _rows(key, "key", (T, Hkv, Dk), dt, dev)
+    v, vs = _rows(value, "value", (T, Hkv, Dv), dt, dev)
+    if state.ndim != 4 or tuple(state.shape[1:]) != (Hkv, Dk, Dv):
+        raise ValueError(f"state must be [slots, {Hkv}, {Dk}, {Dv}], got {list(state.shape)}")
+    if tuple(log_decay.shape) != (Hkv,):
+        raise ValueError(f"log_decay must be [{Hkv}], got {list(log_decay.shape)}")
+    S = state_indices.shape[0]
+    for name, t, n in (("query_start_loc", query_start_loc, S + 1), ("context_lens", context_lens, S), ("state_out_indices", state_out_indices, S)):
+        if t is not None and tuple(t.shape) != (n,):
+            raise ValueError(f"{name} must be [{n}], got {list(t.shape)}")
+    if S == 0 or num_seqs.numel() < 1:
+        raise ValueError("no sequence rows")
+    i32 = torch.int32
+    ptrs = [None if t is None else _on(t, name, kind, dev) for name, t, kind in (
+        ("log_decay", log_decay, torch.float32), ("state", state, torch.float32), ("state_indices", state_indices, i32),
+        ("state_out_indices", state_out_indices, i32), ("context_lens", context_lens, i32), ("query_start_loc", query_start_loc, i32),
+        ("num_seqs", num_seqs, i32))]
+    if out is None:
+        out = torch.empty((T, Hq, Dv), dtype=dt, device=dev)
+    elif tuple(out.shape) != (T, Hq, Dv):
+        raise ValueError(f"out must be [{T}, {Hq}, {Dv}], got {list(out.shape)}")
+    else:
+        a, b = _span(out)
+        for name, t in (("query", query), ("key", key), ("value", value), ("state", state)):
+            c, d = _span(t)
+            if a < d and c < b:
+                raise ValueError(f"out overlaps {name}")
+    o = _on(out, "out", dt, dev)
+    if T > 0:
+        scale = float(Dk) ** -0.5 if scale is None else float(scale)
+        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
+            # scratch of its own for every call: the caching allocator orders its reuse by stream, and a captured graph keeps its own
+            need = int(lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, dtype_tag(dt)))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _lib.check(lib.rpa_decay_linear_attention(
+                _stream(query), q, k, v, *ptrs, o, None if ws is None else ws.data_ptr(), need, T, S, state.shape[0], Hq, Hkv, Dk, Dv,
+                qs, ks, vs, dtype_tag(dt), scale))
+    return out, state

@@ -298,6 +298,100 @@ int rpa_mla_page_scatter(rpa_stream_t stream, const void* keys_values, const voi
                          const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int kv_lora_rank,
                          int qk_rope_head_dim, int row_elems, int elem_bytes);
 
+/*
+ * Append with rotation, ragged form: the write half of the fused v3 operation with the rotary position embedding
+ * applied on the way.  Per query token t of sequence i (placed as by rpa_page_scatter_ragged: cache position
+ * pos = ctx_i - q_len_i + (t - qsl[i])), one launch rotates the query heads into query_out, rotates the key heads into
+ * the pages and copies the value heads into the pages.
+ *
+ *   query, key, value  device, rows of Hq x D, Hkv x D and Hkv x D src_dtype elements (RPA_F32, RPA_BF16, RPA_F16); the heads of
+ *                      a token are contiguous, its rows lie *_stride elements apart (views of one projection's output
+ *                      need no copy); strides >= the row
+ *   query_out          device, [T][Hq][D] src_dtype, contiguous; may be `query` itself if that is contiguous (no other overlap).
+ *                      Rows of padded tokens are written as zeros, and left alone where query_out is query
+ *   kv_pages           device, [P][page_size][C][Dp] kv_dtype, updated in place (elements D..Dp-1 of a written row become
+ *                      zero).  kv_dtype any of the five; int8 only with kv_scales
+ *   kv_scales          device, float [P][C], or NULL.  With scales (8-bit pages) the rotated float32 keys and the values
+ *                      are quantised by the rule of rpa_page_scatter_ragged_quantised, scales updated in place, but for
+ *                      one rounding: the scale that new values ask for is amax * (1 / qmax), the reciprocal rounded to
+ *                      float32 (at most one step from the quotient).  Without scales fp8 pages get the bare cast: round
+ *                      to nearest even, NaN for what rounds beyond 448
+ *   cos_sin            device, float [table_rows][rope_dim]: the cosines of a position's rope_dim / 2 angles, then the sines
+ *   positions          device, int32 [T], or NULL: the table row of each token; NULL: its cache position.  Rows are
+ *                      clamped into [0, table_rows)
+ *   rope_dim           even, <= D: the first rope_dim elements of a head turn, the others are copied
+ *   neox_style         1: element d turns with element d + rope_dim / 2; 0: element 2d with element 2d + 1
+ * For a pair (a, b) and its angle's c, s:  a' = a c - b s,  b' = b c + a s, each product and each sum rounded to float32
+ * (no fused multiply-add, so that the result can be checked bit for bit), then rounded once to the target type.
+ * Positions < 0 and pages outside [0, P) are not written (their queries are still rotated).
+ */
+int rpa_rope_page_scatter_ragged(rpa_stream_t stream, const void* query, const void* key, const void* value, void* query_out,
+                                 void* kv_pages, float* kv_scales, const float* cos_sin, const int32_t* positions,
+                                 const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                                 const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int Hkv, int D,
+                                 int Dp, int C, int rope_dim, int table_rows, int neox_style, int64_t query_stride,
+                                 int64_t key_stride, int64_t value_stride, int src_dtype, int kv_dtype);
+
+/*
+ * The same over separate K and V pools [P][page_size][Hkv][D] (the layout of rpa_unified_attention); no scales, so
+ * kv_dtype is RPA_F32, RPA_BF16, RPA_F16 or RPA_FP8_E4M3 (bare cast).  num_seqs may be NULL: every one of the S rows is live.
+ */
+int rpa_rope_unified_page_scatter(rpa_stream_t stream, const void* query, const void* key, const void* value, void* query_out,
+                                  void* key_cache, void* value_cache, const float* cos_sin, const int32_t* positions,
+                                  const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                                  const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int Hkv, int D,
+                                  int rope_dim, int table_rows, int neox_style, int64_t query_stride, int64_t key_stride,
+                                  int64_t value_stride, int src_dtype, int kv_dtype);
+
+/*
+ * The write half of the multi-latent operation with the rotation applied on the way: queries_pe turn into
+ * queries_pe_out, keys_pe turn into the rope part of the latent rows, keys_values are copied beside them (placement,
+ * padding and limits as for rpa_mla_page_scatter; rotation, table and positions as above, over all
+ * qk_rope_head_dim elements, which must be even).
+ *
+ *   queries_pe    device, rows of Hq x qk_rope_head_dim src_dtype elements, query_stride elements apart
+ *   keys_pe       device, rows of qk_rope_head_dim src_dtype elements, key_stride elements apart
+ *   keys_values   device, [T][kv_lora_rank] kv_dtype, contiguous
+ *   queries_pe_out device, [T][Hq][qk_rope_head_dim] src_dtype; may be a contiguous queries_pe itself
+ */
+int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const void* keys_values, const void* keys_pe,
+                              void* queries_pe_out, void* kv_pages, const float* cos_sin, const int32_t* positions,
+                              const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                              const int32_t* num_seqs, int T, int S, int M, int P, int page_size, int Hq, int kv_lora_rank,
+                              int qk_rope_head_dim, int row_elems, int table_rows, int neox_style, int64_t query_stride,
+                              int64_t key_stride, int src_dtype, int kv_dtype);
+
+/*
+ * Linear attention with one decay per KV head over a ragged batch (prompt chunks and decode rows mixed), its states in
+ * a pool of slots.  For KV head h with decay l = exp(log_decay[h]), sequence i's state S [Dk][Dv] and its tokens in order:
+ *   S <- l S + k_t v_t^T,     out_t = scale * q_t S      for each of the Hq / Hkv query heads that share the state
+ *
+ *   query, key    device, rows of Hq x Dk and Hkv x Dk elements of `dtype` (RPA_F32, RPA_BF16, RPA_F16), heads contiguous,
+ *   value         rows of Hkv x Dv elements; token rows *_stride elements apart
+ *   log_decay     device, float [Hkv], natural log, <= 0 (-inf: nothing is kept).  Not checked: above 0 the state grows
+ *   state         device, float [num_slots][Hkv][Dk][Dv], updated in place
+ *   state_indices device, int32 [S]: the slot that holds sequence i's state before the call
+ *   state_out_indices device, int32 [S], or NULL: the slot its state after the call is written to; NULL: the same slot.
+ *                 Slots written must differ from each other and from the slots other live sequences read
+ *   context_lens  device, int32 [S], or NULL.  A sequence whose context_lens[i] <= q_len_i is fresh: it starts from a zero
+ *                 state whatever its slot holds.  NULL: every sequence goes on from its slot
+ *   query_start_loc device, int32 [S+1]; num_seqs device, int32 [1]
+ *   out           device, [T][Hq][Dv] of `dtype`; rows of padded tokens are written as zeros
+ *   workspace     device, at least rpa_decay_attention_workspace_bytes(...) bytes, 256-byte aligned (NULL if that is 0)
+ * A slot outside [0, num_slots) reads as a zero state and is not written.  Sequences without tokens keep their slots as they are
+ * (nothing is copied to state_out_indices either).  State and sums are float32 throughout.
+ * A value that is not finite reaches its own and later tokens of its sequence only.
+ * Limits: Dk, Dv multiples of 4, at most 256; Hq a multiple of Hkv.
+ */
+int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const void* key, const void* value, const float* log_decay,
+                               float* state, const int32_t* state_indices, const int32_t* state_out_indices,
+                               const int32_t* context_lens, const int32_t* query_start_loc, const int32_t* num_seqs, void* out,
+                               void* workspace, size_t workspace_bytes, int T, int S, int num_slots, int Hq, int Hkv, int Dk,
+                               int Dv, int64_t query_stride, int64_t key_stride, int64_t value_stride, int dtype, float scale);
+
+/* Scratch the call above needs, from the static bounds (and the compute-unit count of the current device). */
+size_t rpa_decay_attention_workspace_bytes(int T, int S, int Hq, int Hkv, int Dk, int Dv, int dtype);
+
 #ifdef __cplusplus
 }
 #endif
