@@ -32,6 +32,7 @@ SOURCES = [
     "rpa_mla.hip",
     "rpa_rope.hip",
     "rpa_decay.hip",
+    "rpa_decay_chunk.hip",
 ]
 # measurement kernels and result-changing test knobs: compiled into the test / benchmark build only (-DRPA_PROBES)
 PROBE_SOURCES = ["rpa_probe.hip"]

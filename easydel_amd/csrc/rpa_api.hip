@@ -927,9 +927,30 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
   return hip_fail(rpa::launch_rope_latent((hipStream_t)stream, p), "rpa_rope_mla_page_scatter launch");
 }
 
+// Segments of the chunked form, from the static bounds: as long as leaves about two workgroups a CU when all T tokens are in
+// use, four chunks of 64 at the least.  scratch: bytes of the states between segments.
+static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayParams& p, size_t* scratch) {
+  const int slices = (Dv + 127) / 128;
+  const int64_t cus = std::max(device_cus(), 1);
+  int64_t len = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus);
+  len = std::max<int64_t>((len + 63) / 64 * 64, 256);
+  p.seg_len = (int)std::min<int64_t>(len, (int64_t)1 << 30);
+  p.slots = T > p.seg_len ? T / p.seg_len + 1 : 0;
+  const int by_token = T / (rpa::kDecayRows + 1) + 1;
+  p.first_by_seq = S <= by_token;
+  p.first_ids = std::min(S, by_token);
+  *scratch = (size_t)2 * p.slots * Hkv * Dk * Dv * 4;
+}
+
 size_t rpa_decay_attention_workspace_bytes(int T, int S, int Hq, int Hkv, int Dk, int Dv, int dtype) {
-  (void)T; (void)S; (void)Hq; (void)Hkv; (void)Dk; (void)Dv; (void)dtype;
-  return 0;
+  if (T <= rpa::kDecayRows || S <= 0 || Hq <= 0 || Hkv <= 0 || Dk <= 0 || Dv <= 0) return 0;
+  rpa::DecayParams p;
+  memset(&p, 0, sizeof(p));
+  p.dtype = dtype;
+  if (!rpa::decay_chunk_supported(p)) return 0;
+  size_t scratch;
+  decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
+  return scratch;
 }
 
 int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const void* key, const void* value, const float* log_decay,
@@ -956,6 +977,7 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   const size_t need = rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, dtype);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(RPA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
+  if (need > 0 && ((uintptr_t)workspace & 15)) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", who);
   rpa::DecayParams p;
   memset(&p, 0, sizeof(p));
   p.q = query; p.k = key; p.v = value; p.log_decay = log_decay; p.state = state;
@@ -963,7 +985,21 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   p.context_lens = context_lens; p.qsl = query_start_loc; p.num_seqs = num_seqs; p.out = out;
   p.T = T; p.S = S; p.num_slots = num_slots; p.Hq = Hq; p.Hkv = Hkv; p.group = Hq / Hkv; p.Dk = Dk; p.Dv = Dv;
   p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.dtype = dtype; p.scale = scale;
-  return hip_fail(rpa::launch_decay_recurrent((hipStream_t)stream, p), "rpa_decay_linear_attention launch");
+  p.rows = T;
+  hipStream_t s = (hipStream_t)stream;
+  if (T > rpa::kDecayRows && rpa::decay_chunk_supported(p)) {
+    size_t scratch;
+    decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
+    p.rows = rpa::kDecayRows;
+    p.scratch = (float*)workspace;
+    const int64_t unit = 16 / e;
+    p.vec = ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)value)) & 15) == 0 && query_stride % unit == 0 && key_stride % unit == 0 &&
+            value_stride % unit == 0 && Dk % unit == 0 && Dv % unit == 0;
+    const int64_t blocks = ((int64_t)p.first_ids + p.slots) * Hkv * 4;
+    if (blocks > INT32_MAX || p.slots > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: T=%d tokens of %d heads are too many workgroups", who, T, Hkv);
+    if (const int err = rpa::launch_decay_chunk(s, p)) return hip_fail(err, "rpa_decay_linear_attention chunk launch");
+  }
+  return hip_fail(rpa::launch_decay_recurrent(s, p), "rpa_decay_linear_attention launch");
 }
 
 }  // extern "C"

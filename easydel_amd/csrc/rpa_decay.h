@@ -20,7 +20,17 @@ struct DecayParams {
   int64_t q_stride, k_stride, v_stride;  // elements
   int dtype;
   float scale;
+  int rows;          // sequences of at most this many tokens take the recurrent form, the others the chunked one (rows >= T: none)
+  // chunked form
+  int vec;           // q, k and v rows allow 16-byte loads
+  int seg_len;       // tokens of a segment
+  int slots;         // scratch slots: floor(T / seg_len) + 1, 0 where no sequence can have two segments
+  int first_ids;     // numbers that first segments may have ...
+  int first_by_seq;  // ... which are their sequences' (1) or floor(qsl[i] / (kDecayRows + 1)) (0)
+  float* scratch;    // [2 * slots][Hkv][Dk][Dv]
 };
+
+constexpr int kDecayRows = 16;
 
 struct DecaySeq {
   int q0, q_len;
@@ -52,6 +62,8 @@ __device__ __forceinline__ float2 decay_power(float g, int n) {
   return make_float2(hi, __builtin_isfinite(hi) ? (float)(e - (double)hi) : 0.f);
 }
 
+bool decay_chunk_supported(const DecayParams& p);
+int launch_decay_chunk(hipStream_t stream, const DecayParams& p);
 int launch_decay_recurrent(hipStream_t stream, const DecayParams& p);
 
 }  // namespace rpa

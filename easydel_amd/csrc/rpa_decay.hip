@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayParams p) {
   const int h = blockIdx.x / slices, c0 = (blockIdx.x - h * slices) * 4 * CG;
   const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
   const DecaySeq s = decay_seq(p, i);
-  if (s.q_len <= 0) return;
+  if (s.q_len <= 0 || s.q_len > p.rows) return;
   const int col = c0 + 4 * cg;
   const bool in_cols = col < p.Dv;
   const int64_t head = (int64_t)p.Dk * p.Dv, at = (int64_t)h * head + col;

@@ -1,0 +1,450 @@
+// Linear attention with one decay per KV head, chunked form, for sequences of more than a few tokens.
+//
+// Within a chunk of C tokens from a state S0, with l = exp(g) and n, m = 0 .. C-1 inside the chunk:
+//     o_n = scale * ( l^(n+1) q_n S0  +  sum_{m <= n} l^(n-m) (q_n . k_m) v_m )
+//     S1  = l^C S0 + sum_m l^(C-1-m) k_m v_m^T
+// No exponent is negative, so nothing overflows that the token-by-token recurrence would not.
+//
+// A sequence is a chain of chunks, which leaves only heads x sequences to work on side by side.  So a long sequence is cut
+// into segments of seg_len tokens: (1) every segment but a sequence's last sums up what it adds to a zero state, (2) a scan
+// turns these into the state ahead of each segment, (3) every segment runs its chunks from there.  (1) and (2) are only
+// launched where the bounds allow a sequence of more than one segment.  The first segments are numbered by sequence or by
+// floor(qsl[i] / (kDecayRows + 1)), the others by floor(qsl[i] / seg_len) + j - 1: both are distinct without a plan, since such
+// a sequence is longer than the divisor.
+#include "rpa_decay.h"
+#include "rpa_mfma.h"
+
+namespace rpa {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Segment {
+  int j, t0, n;      // segment of its sequence, first token, tokens
+  int in, out;       // slots of the sequence
+  int base;          // scratch slot behind its first segment
+  int segments;
+  bool last;
+};
+
+// The segment that scratch slot `slot` lies behind (AHEAD: the one that starts from it).
+template <bool AHEAD>
+__device__ __forceinline__ bool find_by_slot(const DecayParams& p, int slot, Segment& g) {
+  const int n_live = decay_live_rows(p);
+  const int64_t t = (int64_t)slot * p.seg_len + p.seg_len - 1;
+  if (n_live <= 0 || t < p.qsl[0]) return false;
+  // sequences behind one of several segments start at its last segment or later: the last to start up to t owns the slot
+  const int i = find_seq_wave(p.qsl, n_live, (int)min(t, (int64_t)INT32_MAX));
+  const DecaySeq s = decay_seq(p, i);
+  if (s.q_len <= kDecayRows) return false;
+  const int segments = g.segments = (s.q_len + p.seg_len - 1) / p.seg_len;
+  g.base = s.q0 / p.seg_len;
+  g.j = slot - g.base + (AHEAD ? 1 : 0);
+  if (g.j >= segments - (AHEAD ? 0 : 1)) return false;
+  g.t0 = s.q0 + g.j * p.seg_len;
+  g.n = min(s.q_len - g.j * p.seg_len, p.seg_len);
+  g.in = s.in; g.out = s.out;
+  g.last = g.j == segments - 1;
+  return true;
+}
+
+// Segment of workgroup row `id`: ids below p.first_ids are first segments, the others start from a scratch state.
+__device__ __forceinline__ bool find_segment(const DecayParams& p, int id, Segment& g) {
+  if (id >= p.first_ids) return find_by_slot<true>(p, id - p.first_ids, g);
+  const int n_live = decay_live_rows(p);
+  if (n_live <= 0) return false;
+  int i = id;
+  if (!p.first_by_seq) {
+    const int64_t t = (int64_t)id * (kDecayRows + 1) + kDecayRows;
+    if (t < p.qsl[0]) return false;
+    i = find_seq_wave(p.qsl, n_live, (int)min(t, (int64_t)INT32_MAX));
+    if (p.qsl[i] / (kDecayRows + 1) != id) return false;
+  }
+  const DecaySeq s = decay_seq(p, i);
+  if (s.q_len <= kDecayRows) return false;
+  g.j = 0;
+  g.t0 = s.q0;
+  g.n = min(s.q_len, p.seg_len);
+  g.in = s.in; g.out = s.out;
+  g.base = s.q0 / p.seg_len;
+  g.segments = (s.q_len + p.seg_len - 1) / p.seg_len;
+  g.last = g.segments == 1;
+  return true;
+}
+
+__device__ __forceinline__ float* scratch_state(const DecayParams& p, int slot, int h) {
+  return p.scratch + ((int64_t)slot * p.Hkv + h) * p.Dk * p.Dv;
+}
+
+// Where a segment's state comes from (null: zeros).  A sequence of several segments may write the slot it started from while
+// its first segment has yet to run, so the scan keeps the state it starts from, in a second set of scratch slots.
+__device__ __forceinline__ const float* state_ahead(const DecayParams& p, const Segment& g, int h) {
+  if (g.j > 0) return scratch_state(p, g.base + g.j - 1, h);
+  if (!g.last) return scratch_state(p, p.slots + g.base, h);
+  return g.in < 0 ? nullptr : p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv;
+}
+
+// Scratch slots hold what each segment adds to a zero state; afterwards slot base + j holds the state behind segment j.
+__global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
+  Segment g;
+  if (!find_by_slot<false>(p, blockIdx.z, g) || g.j != 0) return;
+  const int h = blockIdx.y, e = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= p.Dk * p.Dv) return;
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g.in >= 0) r = *(const float4*)(p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + e);
+  *(float4*)(scratch_state(p, p.slots + g.base, h) + e) = r;
+  const float2 l = decay_power(p.log_decay[h], p.seg_len);
+  for (int slot = g.base; slot < g.base + g.segments - 1; ++slot) {
+    float4* at = (float4*)(scratch_state(p, slot, h) + e);
+    const float4 a = *at;
+    r.x = fmaf(r.x, l.y, fmaf(r.x, l.x, a.x)); r.y = fmaf(r.y, l.y, fmaf(r.y, l.x, a.y));
+    r.z = fmaf(r.z, l.y, fmaf(r.z, l.x, a.z)); r.w = fmaf(r.w, l.y, fmaf(r.w, l.x, a.w));
+    *at = r;
+  }
+}
+
+// ---- bfloat16: matrix instructions on bf16 operands ---------------------------------------------------------
+// Tiles are 32 x 32 (16 k-values an instruction).  Wave w owns 32 columns of the state and of the output: its part of S stays in
+// accumulators for the whole segment, as tiles of 32 keys-by-columns whose lane half h and register r hold key
+// 32 d + 16 (r / 8) + 8 h + r % 8.  In that order eight registers are one B operand of the product with the queries as
+// they lie in memory; the order comes for free, since the rows of K^T can be read in any order of four.
+//   scores   S^T = K Q^T, three of the four 32 x 32 tiles, shared out over the waves, through LDS as bf16
+//   output   Q S0, rows scaled by l^(n+1) in float32, then + P V
+//   state    l^n S + K^T (l^(n-1-m) V): the decayed values are float32, so they enter as the sum of three bf16 numbers
+//            (24 bits); the state keeps float32 accuracy.
+// Rounded to bf16 are the scores and, for Q S0 only, the state: what they add to an output is rounded to bf16 as well.
+
+constexpr int kChunk = 64;
+constexpr int kStrip = 80;  // bytes of a row of a wave's 32 output columns in LDS, spread over the banks
+
+// 16-byte chunks of a row of NCH of them are stored XOR-ed with this key: eight consecutive rows read at one chunk, and four
+// rows read at a pair of chunks by the transposing loads, fall on distinct banks.
+template <int WIDTH>
+__device__ __forceinline__ int tile_key(int row) {
+  if constexpr (WIDTH >= 128) return (row & 7) << 1;
+  else return ((row >> 1) & 3) << 1;
+}
+
+template <int WIDTH>
+__device__ __forceinline__ u32x4 row_operand(const char* tile, int row, int chunk) {
+  return *(const u32x4*)(tile + row * WIDTH * 2 + ((chunk ^ tile_key<WIDTH>(row)) << 4));
+}
+
+// Four rows from `row` of column col + (lane & 15), where the lane supplies the address of row row + (lane & 15) / 4 and its own
+// four columns `mine`.
+template <int WIDTH>
+__device__ __forceinline__ u32x2 column_operand(const char* tile, int row, int mine) {
+  const int r = row + ((threadIdx.x & 15) >> 2);
+  const char* a = tile + r * WIDTH * 2 + (((mine >> 3) ^ tile_key<WIDTH>(r)) << 4) + ((mine & 7) << 1);
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)a));
+}
+
+__device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Rows of a tile on their way from memory to LDS, 16 bytes a piece; a thread's pieces lie ROWS rows apart.
+template <int WIDTH, int NT>
+struct Stage {
+  static constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT, ROWS = NT / PER_ROW;
+  u32x4 r[N];
+  // rows 0 .. n-1 of `src` (`stride` elements apart, `cols` elements each); zeros elsewhere.  vec: 16-byte loads allowed.
+  __device__ __forceinline__ void load(const uint16_t* src, int64_t stride, int n, int cols, bool vec) {
+    const int row = threadIdx.x / PER_ROW, c = (threadIdx.x % PER_ROW) * 8;
+    const uint32_t at = ((uint32_t)row * (uint32_t)stride + c) * 2;  // 64 rows span less than 2^31 bytes
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const char* s = (const char*)(src + k * ROWS * stride);
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (row + k * ROWS < n && c < cols) {
+        if (vec) {
+          v = *(const u32x4*)(s + at);
+        } else {
+          uint64_t lo = 0, hi = 0;  // element by element, low to high
+#pragma unroll 1
+          for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
+            hi = (hi << 16) | (lo >> 48);
+            lo = (lo << 16) | *(const uint16_t*)(s + at + 2 * x);
+          }
+          v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        }
+      }
+      r[k] = v;
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+    const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW;
+#pragma unroll
+    for (int k = 0; k < N; ++k) *(u32x4*)(tile + (row + k * ROWS) * WIDTH * 2 + ((c ^ tile_key<WIDTH>(row + k * ROWS)) << 4)) = r[k];
+  }
+};
+
+// Eight decayed values as three bf16 operands whose sum is the float32 value.
+__device__ __forceinline__ void split3(u32x4 v, const float4& w0, const float4& w1, u32x4& hi, u32x4& mid, u32x4& lo) {
+  const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = low_half(v[i]) * w[2 * i], b = high_half(v[i]) * w[2 * i + 1];
+    hi[i] = pack_bf16(a, b);
+    a -= low_half(hi[i]); b -= high_half(hi[i]);
+    mid[i] = pack_bf16(a, b);
+    a -= low_half(mid[i]); b -= high_half(mid[i]);
+    lo[i] = pack_bf16(a, b);
+  }
+}
+
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+  return w;
+}
+
+template <int DK, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
+  constexpr int NT = 64 * NW, DV = 32 * NW, ND = DK / 32;
+  __shared__ __align__(16) char sQ[OUT ? kChunk * DK * 2 : 16];
+  __shared__ __align__(16) char sK[kChunk * DK * 2];
+  __shared__ __align__(16) char sV[kChunk * DV * 2];
+  __shared__ __align__(16) char sP[OUT ? kChunk * kChunk * 2 : 16];
+  __shared__ __align__(16) char sO[OUT ? NW * kChunk * kStrip : 16];
+  __shared__ __align__(16) float pw[kChunk + 4];  // l^0 .. l^C
+  __shared__ __align__(16) float left[kChunk];    // l^(n-1-m) for the n tokens m of a chunk, 0 behind them
+  __shared__ float2 whole[2];                     // l^n of a full chunk and of the last one, as two floats
+
+  const int slices = (p.Dv + DV - 1) / DV, heads = p.Hkv * slices;
+  const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
+  Segment g;
+  if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5;
+  int l31 = lane & 31;
+  const int chunks = (g.n + kChunk - 1) / kChunk, tail = g.n - (chunks - 1) * kChunk;
+  const float rate = p.log_decay[h];
+  if (tid <= kChunk) pw[tid] = decay_power(rate, tid).x;
+  else if (tid < kChunk + 3) whole[tid - kChunk - 1] = decay_power(rate, tid == kChunk + 1 ? kChunk : tail);
+  if (tid < kChunk) left[tid] = decay_power(rate, kChunk - 1 - tid).x;
+
+  const int col = c0 + 32 * w + l31;
+  const bool mine = col < p.Dv;
+  f32x16 S[ND];
+  const float* from = OUT ? state_ahead(p, g, h) : nullptr;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) S[d] = f32x16{};
+  if (from != nullptr && mine) {
+    const float* at = from + 8 * half * p.Dv + col;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = 32 * d + 16 * (r >> 3) + (r & 7);
+        if (key + 8 * half < p.Dk) S[d][r] = at[key * p.Dv];
+      }
+  }
+
+  const uint16_t* q = (const uint16_t*)p.q + (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk;
+  const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
+  const uint16_t* v = (const uint16_t*)p.v + (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
+  const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
+  Stage<DK, NT> nq, nk;
+  Stage<DV, NT> nv;
+  if (OUT) nq.load(q, p.q_stride, g.n, p.Dk, p.vec);
+  nk.load(k, p.k_stride, g.n, p.Dk, p.vec);
+  nv.load(v, p.v_stride, g.n, vcols, p.vec);
+  const int vcol = 32 * w + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);                            // this lane's share of the transposing loads
+  const int kcol = 16 * ((lane >> 4) & 1) + 4 * (((lane & 1) << 1) | ((lane >> 1) & 1));
+
+  for (int c = 0; c < chunks; ++c) {
+    const int n = min(g.n - c * kChunk, kChunk);
+    for (int gq = 0; gq < groups; ++gq) {
+      __syncthreads();  // the tiles of the step before have been read
+      if (OUT) nq.store(sQ);
+      if (gq == 0) {
+        nk.store(sK);
+        nv.store(sV);
+        if (n < kChunk && tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;
+      }
+      __syncthreads();
+      const bool on = gq == groups - 1;  // the next step is another chunk's
+      const int cn = c + (on ? 1 : 0);
+      const int64_t ahead = (int64_t)cn * kChunk;
+      if (cn < chunks) {
+        if (OUT) nq.load(q + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), p.q_stride, g.n - cn * kChunk, p.Dk, p.vec);
+        if (on) {
+          nk.load(k + ahead * p.k_stride, p.k_stride, g.n - cn * kChunk, p.Dk, p.vec);
+          nv.load(v + ahead * p.v_stride, p.v_stride, g.n - cn * kChunk, vcols, p.vec);
+        }
+      }
+      // l31 as the compiler cannot know it is the same in every step: what it derives from it (masks, table addresses) is
+      // then worked out where it is used and not held in registers across the loop
+      asm volatile("" : "+v"(l31));
+      if constexpr (OUT) {
+        // scores, decayed and masked: tile (keys 32 a.., queries 32 b..) of S^T
+#pragma unroll
+        for (int tile = 0; tile < 3; ++tile) {
+          if (tile % NW != w) continue;
+          const int a = tile == 1 ? 1 : 0, b = tile == 0 ? 0 : 1;
+          f32x16 acc = {};
+#pragma unroll
+          for (int ks = 0; ks < DK / 16; ++ks)
+            acc = mfma_bf16(row_operand<DK>(sK, 32 * a + l31, 2 * ks + half), row_operand<DK>(sQ, 32 * b + l31, 2 * ks + half), acc);
+          const int t = 32 * b + l31;
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int s0 = 32 * a + 8 * r4 + 4 * half;
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int gap = t - s0 - e;
+              f[e] = gap >= 0 ? acc[4 * r4 + e] * pw[gap >= 0 ? gap : 0] : 0.f;  // chosen, not multiplied: masked scores may be infinite
+            }
+            const u32x2 two = {pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
+            *(u32x2*)(sP + t * kChunk * 2 + (((s0 >> 3) ^ (t & 7)) << 4) + ((s0 & 7) << 1)) = two;
+          }
+        }
+        __syncthreads();
+        u32x4 vop[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const u32x2 x = column_operand<DV>(sV, 16 * ks + 8 * half, vcol), y = column_operand<DV>(sV, 16 * ks + 8 * half + 4, vcol);
+          vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
+        }
+        f32x16 o[2];  // of the transposed output: lane = token, registers = columns 8 (r / 4) + 4 half + r % 4
+        const float ahead_of[2] = {pw[l31 + 1], pw[32 + l31 + 1]};
+        // A value that is not finite would meet the zeros of the masked scores as well, and 0 x Inf is NaN: such values stay out of
+        // the product, and the rows that see one become NaN by hand.
+        uint32_t full = 0;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) full |= (vop[ks][x] & 0x7f807f80u) + 0x00800080u;  // bit 15 or 31: an exponent of all ones
+        const bool odd = __any((full & 0x80008000u) != 0);
+        if (odd) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) vop[ks][x] = finite_halves(vop[ks][x]);
+        }
+        o[0] = f32x16{}; o[1] = f32x16{};
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const u32x4 s = {pack_bf16(S[d][8 * x], S[d][8 * x + 1]), pack_bf16(S[d][8 * x + 2], S[d][8 * x + 3]),
+                             pack_bf16(S[d][8 * x + 4], S[d][8 * x + 5]), pack_bf16(S[d][8 * x + 6], S[d][8 * x + 7])};
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(s, row_operand<DK>(sQ, 32 * tt + l31, 4 * d + 2 * x + half), o[tt]);
+          }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[tt][r] *= ahead_of[tt];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int tt = ks >> 1; tt < 2; ++tt) {
+            const int t = 32 * tt + l31;
+            o[tt] = mfma_bf16(vop[ks], *(const u32x4*)(sP + t * kChunk * 2 + (((2 * ks + half) ^ (t & 7)) << 4)), o[tt]);
+          }
+        char* strip = sO + w * kChunk * kStrip;  // this wave's 64 rows of 32 columns
+        if (odd) {
+          const int at = 32 * w + l31;
+          int bad = 0;
+          for (; bad < n; ++bad) {
+            const uint16_t bits = *(const uint16_t*)(sV + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
+            if ((bits & 0x7f80) == 0x7f80) break;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int first = __shfl(bad, 8 * (r >> 2) + 4 * half + (r & 3));
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) o[tt][r] = 32 * tt + l31 >= first ? __builtin_nanf("") : o[tt][r];
+          }
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const u32x2 two = {pack_bf16(o[tt][4 * r4] * p.scale, o[tt][4 * r4 + 1] * p.scale),
+                               pack_bf16(o[tt][4 * r4 + 2] * p.scale, o[tt][4 * r4 + 3] * p.scale)};
+            *(u32x2*)(strip + (32 * tt + l31) * kStrip + 16 * r4 + 8 * half) = two;
+          }
+        __builtin_amdgcn_wave_barrier();  // the strip is this wave's own: its LDS accesses stay in order
+        char* out = (char*)p.out + (((int64_t)(g.t0 + c * kChunk) * p.Hq + h * p.group + gq) * p.Dv + c0 + 32 * w) * 2;
+        const int piece = lane & 3, cols = p.Dv - c0 - 32 * w - 8 * piece;  // columns of the piece that exist
+        for (int row = lane >> 2; row < n; row += 16) {
+          const u32x4 v8 = *(const u32x4*)(strip + row * kStrip + 16 * piece);
+          char* to = out + (int64_t)row * p.Hq * p.Dv * 2 + 16 * piece;
+          if (cols >= 8 && (p.Dv & 7) == 0) *(u32x4*)to = v8;
+          else if (cols >= 4) { *(u32x2*)to = u32x2{v8[0], v8[1]}; if (cols >= 8) *(u32x2*)(to + 8) = u32x2{v8[2], v8[3]}; }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    if (OUT && c == chunks - 1 && (!g.last || g.out < 0)) break;  // nobody reads the state behind this chunk
+    const float2 l = whole[n < kChunk ? 1 : 0];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[d][r] = fmaf(S[d][r], l.y, S[d][r] * l.x);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const int m = 16 * ks + 8 * half;
+      const u32x2 x = column_operand<DV>(sV, m, vcol), y = column_operand<DV>(sV, m + 4, vcol);
+      u32x4 hi, mid, lo;
+      split3(u32x4{x[0], x[1], y[0], y[1]}, *(const float4*)&left[m], *(const float4*)&left[m + 4], hi, mid, lo);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const u32x2 u = column_operand<DK>(sK, m, 32 * d + kcol), z = column_operand<DK>(sK, m + 4, 32 * d + kcol);
+        const u32x4 kt = {u[0], u[1], z[0], z[1]};
+        S[d] = mfma_bf16(kt, lo, S[d]);
+        S[d] = mfma_bf16(kt, mid, S[d]);
+        S[d] = mfma_bf16(kt, hi, S[d]);
+      }
+    }
+  }
+  if (OUT && (!g.last || g.out < 0)) return;
+  float* to = OUT ? p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv : scratch_state(p, g.base + g.j, h);
+  int back = 8 * half;
+  asm volatile("" : "+v"(back));  // the addresses and masks are not those of the beginning, kept through the loop
+  if (!mine) return;
+  float* at = to + back * p.Dv + col;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = 32 * d + 16 * (r >> 3) + (r & 7);
+      if (key + back < p.Dk) at[key * p.Dv] = S[d][r];
+    }
+}
+
+template <int DK, int NW>
+void launch_bf16(hipStream_t stream, const DecayParams& p) {
+  const int slices = (p.Dv + 32 * NW - 1) / (32 * NW), heads = p.Hkv * slices;
+  if (p.slots > 0) {
+    hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), dim3(p.slots * heads), dim3(64 * NW), 0, stream, p);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
+  }
+  hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true>), dim3((p.first_ids + p.slots) * heads), dim3(64 * NW), 0, stream, p);
+}
+
+template <int DK>
+void launch_bf16_cols(hipStream_t stream, const DecayParams& p) {
+  if (p.Dv <= 64) launch_bf16<DK, 2>(stream, p);
+  else launch_bf16<DK, 4>(stream, p);
+}
+
+}  // namespace
+
+bool decay_chunk_supported(const DecayParams& p) { return p.dtype == RPA_BF16; }
+
+int launch_decay_chunk(hipStream_t stream, const DecayParams& p) {
+  if (p.Dk <= 64) launch_bf16_cols<64>(stream, p);
+  else if (p.Dk <= 128) launch_bf16_cols<128>(stream, p);
+  else launch_bf16_cols<256>(stream, p);
+  return (int)hipGetLastError();
+}
+
+}  // namespace rpa
