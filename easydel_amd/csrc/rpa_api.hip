@@ -987,7 +987,9 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.dtype = dtype; p.scale = scale;
   p.rows = T;
   hipStream_t s = (hipStream_t)stream;
-  if (T > rpa::kDecayRows && rpa::decay_chunk_supported(p)) {
+  // (rows that lie 2^23 elements apart would pass the chunked form's 32-bit offsets in a chunk: the recurrent form takes them)
+  const bool near = std::max(query_stride, std::max(key_stride, value_stride)) < ((int64_t)1 << 23);
+  if (T > rpa::kDecayRows && near && rpa::decay_chunk_supported(p)) {
     size_t scratch;
     decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
     p.rows = rpa::kDecayRows;

@@ -105,20 +105,22 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
 }
 
 // ---- bfloat16: matrix instructions on bf16 operands ---------------------------------------------------------
-// Tiles are 32 x 32 (16 k-values an instruction).  Wave w owns 32 columns of the state and of the output: its part of S stays in
-// accumulators for the whole segment, as tiles of 32 keys-by-columns whose lane half h and register r hold key
-// 32 d + 16 (r / 8) + 8 h + r % 8.  In that order eight registers are one B operand of the product with the queries as
-// they lie in memory; the order comes for free, since the rows of K^T can be read in any order of four.
-//   scores   S^T = K Q^T, three of the four 32 x 32 tiles, shared out over the waves, through LDS as bf16
-//   output   Q S0, rows scaled by l^(n+1) in float32, then + P V
+// Chunks of 32 tokens.  Wave w owns 32 columns of the state and of the output: its part of S stays in accumulators for the whole
+// segment, as 32 x 32 tiles whose lane half h and register r hold key 32 d + 16 (r / 8) + 8 h + r % 8.  In that order eight
+// registers, rounded to bf16, are one operand of the product with the queries as they lie in memory; the order comes for free,
+// since the rows of K^T can be read in any order of four.
+//   scores   S^T = K Q^T, three of the four 16 x 16 tiles, shared out over the waves, through LDS as bf16
+//   output   O^T = S0^T Q^T, columns scaled by l^(n+1) in float32, then + V^T P^T
 //   state    l^n S + K^T (l^(n-1-m) V): the decayed values are float32, so they enter as the sum of three bf16 numbers
 //            (24 bits); the state keeps float32 accuracy.
-// Rounded to bf16 are the scores and, for Q S0 only, the state: what they add to an output is rounded to bf16 as well.
+// Rounded to bf16 are the scores and, for the product with the queries only, the state: what they add to an output is rounded
+// to bf16 as well.  The tiles of the next chunk are on their way into LDS (direct loads, two buffers) while this one is worked on;
+// registers hold no tile in flight, so two workgroups share a CU and fill each other's waits.
 
-constexpr int kChunk = 64;
-constexpr int kStrip = 80;  // bytes of a row of a wave's 32 output columns in LDS, spread over the banks
+constexpr int kChunk = 32;
+constexpr int kStrip = 80;  // bytes of a row of 32 bf16 values in LDS, spread over the banks
 
-// 16-byte chunks of a row of NCH of them are stored XOR-ed with this key: eight consecutive rows read at one chunk, and four
+// 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key: eight consecutive rows read at one chunk, and four
 // rows read at a pair of chunks by the transposing loads, fall on distinct banks.
 template <int WIDTH>
 __device__ __forceinline__ int tile_key(int row) {
@@ -126,18 +128,21 @@ __device__ __forceinline__ int tile_key(int row) {
   else return ((row >> 1) & 3) << 1;
 }
 
+typedef __attribute__((address_space(3))) const char lds_char;
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
+
 template <int WIDTH>
 __device__ __forceinline__ u32x4 row_operand(const char* tile, int row, int chunk) {
   return *(const u32x4*)(tile + row * WIDTH * 2 + ((chunk ^ tile_key<WIDTH>(row)) << 4));
 }
 
-// Four rows from `row` of column col + (lane & 15), where the lane supplies the address of row row + (lane & 15) / 4 and its own
-// four columns `mine`.
+// Four rows from `row` on of sixteen columns, one column a lane (of each group of sixteen): the lane supplies the address of row
+// row + (lane & 15) / 4 and of the four columns `mine` on that lanes 4 (lane & 3) .. + 3 are to hold.
 template <int WIDTH>
 __device__ __forceinline__ u32x2 column_operand(const char* tile, int row, int mine) {
   const int r = row + ((threadIdx.x & 15) >> 2);
   const char* a = tile + r * WIDTH * 2 + (((mine >> 3) ^ tile_key<WIDTH>(r)) << 4) + ((mine & 7) << 1);
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)a));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds_address(a)));
 }
 
 __device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
@@ -147,41 +152,38 @@ __device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// Rows of a tile on their way from memory to LDS, 16 bytes a piece; a thread's pieces lie ROWS rows apart.
-template <int WIDTH, int NT>
-struct Stage {
-  static constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT, ROWS = NT / PER_ROW;
-  u32x4 r[N];
-  // rows 0 .. n-1 of `src` (`stride` elements apart, `cols` elements each); zeros elsewhere.  vec: 16-byte loads allowed.
-  __device__ __forceinline__ void load(const uint16_t* src, int64_t stride, int n, int cols, bool vec) {
-    const int row = threadIdx.x / PER_ROW, c = (threadIdx.x % PER_ROW) * 8;
-    const uint32_t at = ((uint32_t)row * (uint32_t)stride + c) * 2;  // 64 rows span less than 2^31 bytes
+__device__ uint4 decay_zeros;  // 16 bytes of zeros: the source of what a tile holds beyond its rows and columns
+
+// Starts a tile of kChunk rows of WIDTH elements on its way into LDS; rows 0 .. n-1 of `cols` elements exist, `stride` elements
+// apart, the others become zeros.  VEC: direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's
+// vector-memory counter says so.  Otherwise rows at any address, element by element, complete at the next barrier.
+template <int WIDTH, int NT, bool VEC>
+__device__ __forceinline__ void start_tile(char* tile, const uint16_t* src, int64_t stride, int n, int cols) {
+  constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT;
+  static_assert(N >= 1, "at least one piece a thread");
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const char* s = (const char*)(src + k * ROWS * stride);
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (row + k * ROWS < n && c < cols) {
-        if (vec) {
-          v = *(const u32x4*)(s + at);
-        } else {
-          uint64_t lo = 0, hi = 0;  // element by element, low to high
+  for (int k = 0; k < N; ++k) {
+    // wave w's instruction k fills bytes [(w N + k) 1024, + 1024) of the tile
+    const int piece = ((threadIdx.x >> 6) * N + k) * 64 + (threadIdx.x & 63), row = piece / PER_ROW;
+    const int c = ((piece % PER_ROW) ^ tile_key<WIDTH>(row)) * 8;
+    if constexpr (VEC) {
+      const void* at = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + ((threadIdx.x >> 6) * N + k) * 1024);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+    } else {
+      uint64_t lo = 0, hi = 0;
+      if (row < n) {
+        const uint16_t* at = src + row * stride + c;
 #pragma unroll 1
-          for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
-            hi = (hi << 16) | (lo >> 48);
-            lo = (lo << 16) | *(const uint16_t*)(s + at + 2 * x);
-          }
-          v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
+          hi = (hi << 16) | (lo >> 48);
+          lo = (lo << 16) | at[x];
         }
       }
-      r[k] = v;
+      *(u32x4*)(tile + piece * 16) = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
   }
-  __device__ __forceinline__ void store(char* tile) const {
-    const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW;
-#pragma unroll
-    for (int k = 0; k < N; ++k) *(u32x4*)(tile + (row + k * ROWS) * WIDTH * 2 + ((c ^ tile_key<WIDTH>(row + k * ROWS)) << 4)) = r[k];
-  }
-};
+}
 
 // Eight decayed values as three bf16 operands whose sum is the float32 value.
 __device__ __forceinline__ void split3(u32x4 v, const float4& w0, const float4& w1, u32x4& hi, u32x4& mid, u32x4& lo) {
@@ -203,13 +205,14 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return w;
 }
 
-template <int DK, int NW, bool OUT>
+template <int DK, int NW, bool OUT, bool VEC>
 __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
   constexpr int NT = 64 * NW, DV = 32 * NW, ND = DK / 32;
-  __shared__ __align__(16) char sQ[OUT ? kChunk * DK * 2 : 16];
-  __shared__ __align__(16) char sK[kChunk * DK * 2];
-  __shared__ __align__(16) char sV[kChunk * DV * 2];
-  __shared__ __align__(16) char sP[OUT ? kChunk * kChunk * 2 : 16];
+  constexpr int KB = kChunk * DK * 2, VB = kChunk * DV * 2;
+  __shared__ __align__(1024) char sK[2][KB];
+  __shared__ __align__(1024) char sV[2][VB];
+  __shared__ __align__(1024) char sQ[OUT ? 2 : 1][OUT ? KB : 16];
+  __shared__ __align__(16) char sP[OUT ? kChunk * kStrip : 16];
   __shared__ __align__(16) char sO[OUT ? NW * kChunk * kStrip : 16];
   __shared__ __align__(16) float pw[kChunk + 4];  // l^0 .. l^C
   __shared__ __align__(16) float left[kChunk];    // l^(n-1-m) for the n tokens m of a chunk, 0 behind them
@@ -219,13 +222,23 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
   const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
   Segment g;
   if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5;
-  int l31 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, l31 = lane & 31;
   const int chunks = (g.n + kChunk - 1) / kChunk, tail = g.n - (chunks - 1) * kChunk;
+  const uint16_t* q = (const uint16_t*)p.q + (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk;
+  const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
+  const uint16_t* v = (const uint16_t*)p.v + (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
+  const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
+  start_tile<DK, NT, VEC>(sK[0], k, p.k_stride, g.n, p.Dk);
+  start_tile<DV, NT, VEC>(sV[0], v, p.v_stride, g.n, vcols);
+  if constexpr (OUT) start_tile<DK, NT, VEC>(sQ[0], q, p.q_stride, g.n, p.Dk);
+
   const float rate = p.log_decay[h];
   if (tid <= kChunk) pw[tid] = decay_power(rate, tid).x;
   else if (tid < kChunk + 3) whole[tid - kChunk - 1] = decay_power(rate, tid == kChunk + 1 ? kChunk : tail);
-  if (tid < kChunk) left[tid] = decay_power(rate, kChunk - 1 - tid).x;
+  if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_power(rate, kChunk - 1 - (tid - 64)).x;
+  if constexpr (OUT) {
+    if (tid < 64) *(u32x4*)(sP + (tid & 15) * kStrip + 32 + (tid >> 4 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};  // the tile of masked scores alone
+  }
 
   const int col = c0 + 32 * w + l31;
   const bool mine = col < p.Dv;
@@ -233,145 +246,120 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
   const float* from = OUT ? state_ahead(p, g, h) : nullptr;
 #pragma unroll
   for (int d = 0; d < ND; ++d) S[d] = f32x16{};
-  if (from != nullptr && mine) {
-    const float* at = from + 8 * half * p.Dv + col;
+  if (from != nullptr) {
+    const float* at = from + (mine ? col : 0);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int key = 32 * d + 16 * (r >> 3) + (r & 7);
-        if (key + 8 * half < p.Dk) S[d][r] = at[key * p.Dv];
+        const int key = 32 * d + 16 * (r >> 3) + 8 * half + (r & 7);
+        const float x = at[min(key, p.Dk - 1) * p.Dv];  // unconditional loads, all in flight at once
+        S[d][r] = mine && key < p.Dk ? x : 0.f;
       }
   }
 
-  const uint16_t* q = (const uint16_t*)p.q + (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk;
-  const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
-  const uint16_t* v = (const uint16_t*)p.v + (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
-  const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
-  Stage<DK, NT> nq, nk;
-  Stage<DV, NT> nv;
-  if (OUT) nq.load(q, p.q_stride, g.n, p.Dk, p.vec);
-  nk.load(k, p.k_stride, g.n, p.Dk, p.vec);
-  nv.load(v, p.v_stride, g.n, vcols, p.vec);
-  const int vcol = 32 * w + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);                            // this lane's share of the transposing loads
+  // this lane's share of the transposing loads
+  const int vcol = 32 * w + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const int kcol = 16 * ((lane >> 4) & 1) + 4 * (((lane & 1) << 1) | ((lane >> 1) & 1));
 
   for (int c = 0; c < chunks; ++c) {
     const int n = min(g.n - c * kChunk, kChunk);
+    const char *tK = sK[c & 1], *tV = sV[c & 1];
+    u32x4 vop[2];
     for (int gq = 0; gq < groups; ++gq) {
-      __syncthreads();  // the tiles of the step before have been read
-      if (OUT) nq.store(sQ);
-      if (gq == 0) {
-        nk.store(sK);
-        nv.store(sV);
-        if (n < kChunk && tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;
-      }
+      const int step = c * groups + gq;
+      // this step's tiles have arrived (so have the output rows of the step before), and the other buffers have been read
+      if constexpr (VEC) wait_loads<0>();
       __syncthreads();
       const bool on = gq == groups - 1;  // the next step is another chunk's
       const int cn = c + (on ? 1 : 0);
-      const int64_t ahead = (int64_t)cn * kChunk;
       if (cn < chunks) {
-        if (OUT) nq.load(q + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), p.q_stride, g.n - cn * kChunk, p.Dk, p.vec);
+        const int64_t ahead = (int64_t)cn * kChunk;
+        if constexpr (OUT) start_tile<DK, NT, VEC>(sQ[(step + 1) & 1], q + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), p.q_stride, g.n - cn * kChunk, p.Dk);
         if (on) {
-          nk.load(k + ahead * p.k_stride, p.k_stride, g.n - cn * kChunk, p.Dk, p.vec);
-          nv.load(v + ahead * p.v_stride, p.v_stride, g.n - cn * kChunk, vcols, p.vec);
+          start_tile<DK, NT, VEC>(sK[cn & 1], k + ahead * p.k_stride, p.k_stride, g.n - cn * kChunk, p.Dk);
+          start_tile<DV, NT, VEC>(sV[cn & 1], v + ahead * p.v_stride, p.v_stride, g.n - cn * kChunk, vcols);
         }
       }
-      // l31 as the compiler cannot know it is the same in every step: what it derives from it (masks, table addresses) is
-      // then worked out where it is used and not held in registers across the loop
-      asm volatile("" : "+v"(l31));
+      if (n < kChunk && gq == 0) {  // the last chunk alone
+        if (tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;
+        if constexpr (!OUT) __syncthreads();
+      }
       if constexpr (OUT) {
-        // scores, decayed and masked: tile (keys 32 a.., queries 32 b..) of S^T
+        const char* tQ = sQ[step & 1];
+        // scores, decayed and masked: tile (keys 16 a.., queries 16 b..) of S^T
+        const int i16 = lane & 15, g4 = lane >> 4;
 #pragma unroll
         for (int tile = 0; tile < 3; ++tile) {
           if (tile % NW != w) continue;
           const int a = tile == 1 ? 1 : 0, b = tile == 0 ? 0 : 1;
-          f32x16 acc = {};
+          f32x4 acc = {};
 #pragma unroll
-          for (int ks = 0; ks < DK / 16; ++ks)
-            acc = mfma_bf16(row_operand<DK>(sK, 32 * a + l31, 2 * ks + half), row_operand<DK>(sQ, 32 * b + l31, 2 * ks + half), acc);
-          const int t = 32 * b + l31;
+          for (int ks = 0; ks < DK / 32; ++ks)
+            acc = HalfOf<RPA_BF16>::mfma32(row_operand<DK>(tK, 16 * a + i16, 4 * ks + g4), row_operand<DK>(tQ, 16 * b + i16, 4 * ks + g4), acc);
+          const int t = 16 * b + i16, s0 = 16 * a + 4 * g4;
+          float f[4];
 #pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const int s0 = 32 * a + 8 * r4 + 4 * half;
-            float f[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int gap = t - s0 - e;
-              f[e] = gap >= 0 ? acc[4 * r4 + e] * pw[gap >= 0 ? gap : 0] : 0.f;  // chosen, not multiplied: masked scores may be infinite
-            }
-            const u32x2 two = {pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
-            *(u32x2*)(sP + t * kChunk * 2 + (((s0 >> 3) ^ (t & 7)) << 4) + ((s0 & 7) << 1)) = two;
+          for (int e = 0; e < 4; ++e) {
+            const int gap = t - s0 - e;
+            f[e] = gap >= 0 ? acc[e] * pw[max(gap, 0)] : 0.f;  // chosen, not multiplied: masked scores may be infinite
           }
+          *(u32x2*)(sP + t * kStrip + s0 * 2) = u32x2{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
         }
         __syncthreads();
-        u32x4 vop[4];
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const u32x2 x = column_operand<DV>(sV, 16 * ks + 8 * half, vcol), y = column_operand<DV>(sV, 16 * ks + 8 * half + 4, vcol);
-          vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
-        }
-        f32x16 o[2];  // of the transposed output: lane = token, registers = columns 8 (r / 4) + 4 half + r % 4
-        const float ahead_of[2] = {pw[l31 + 1], pw[32 + l31 + 1]};
-        // A value that is not finite would meet the zeros of the masked scores as well, and 0 x Inf is NaN: such values stay out of
-        // the product, and the rows that see one become NaN by hand.
-        uint32_t full = 0;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) full |= (vop[ks][x] & 0x7f807f80u) + 0x00800080u;  // bit 15 or 31: an exponent of all ones
-        const bool odd = __any((full & 0x80008000u) != 0);
-        if (odd) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) vop[ks][x] = finite_halves(vop[ks][x]);
-        }
-        o[0] = f32x16{}; o[1] = f32x16{};
+        // O^T of this wave's columns: lane = token, registers = columns 8 (r / 4) + 4 half + r % 4
+        f32x16 o = {};
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const u32x4 s = {pack_bf16(S[d][8 * x], S[d][8 * x + 1]), pack_bf16(S[d][8 * x + 2], S[d][8 * x + 3]),
                              pack_bf16(S[d][8 * x + 4], S[d][8 * x + 5]), pack_bf16(S[d][8 * x + 6], S[d][8 * x + 7])};
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(s, row_operand<DK>(sQ, 32 * tt + l31, 4 * d + 2 * x + half), o[tt]);
+            o = mfma_bf16(s, row_operand<DK>(tQ, l31, 4 * d + 2 * x + half), o);
           }
+        const float ahead_of = pw[l31 + 1];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int r = 0; r < 16; ++r) o[r] *= ahead_of;
+        // A value that is not finite would meet the zeros of the masked scores as well, and 0 x Inf is NaN: such values stay out of
+        // the product, and the rows that see one become NaN by hand.
+        uint32_t full = 0;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[tt][r] *= ahead_of[tt];
+        for (int ks = 0; ks < 2; ++ks) {
+          const u32x2 x = column_operand<DV>(tV, 16 * ks + 8 * half, vcol), y = column_operand<DV>(tV, 16 * ks + 8 * half + 4, vcol);
+          vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+          for (int e = 0; e < 4; ++e) full |= (vop[ks][e] & 0x7f807f80u) + 0x00800080u;  // bit 15 or 31: an exponent of all ones
+        }
+        const bool odd = __any((full & 0x80008000u) != 0);
 #pragma unroll
-          for (int tt = ks >> 1; tt < 2; ++tt) {
-            const int t = 32 * tt + l31;
-            o[tt] = mfma_bf16(vop[ks], *(const u32x4*)(sP + t * kChunk * 2 + (((2 * ks + half) ^ (t & 7)) << 4)), o[tt]);
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4 vo = vop[ks];
+          if (odd) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vo[e] = finite_halves(vo[e]);
           }
-        char* strip = sO + w * kChunk * kStrip;  // this wave's 64 rows of 32 columns
+          o = mfma_bf16(vo, *(const u32x4*)(sP + l31 * kStrip + (2 * ks + half) * 16), o);
+        }
         if (odd) {
           const int at = 32 * w + l31;
           int bad = 0;
           for (; bad < n; ++bad) {
-            const uint16_t bits = *(const uint16_t*)(sV + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
+            const uint16_t bits = *(const uint16_t*)(tV + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
             if ((bits & 0x7f80) == 0x7f80) break;
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int first = __shfl(bad, 8 * (r >> 2) + 4 * half + (r & 3));
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) o[tt][r] = 32 * tt + l31 >= first ? __builtin_nanf("") : o[tt][r];
+            o[r] = l31 >= first ? __builtin_nanf("") : o[r];
           }
         }
+        // through this wave's own strip of LDS (whose accesses stay in order) to whole rows of 32 columns
+        char* strip = sO + w * kChunk * kStrip;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const u32x2 two = {pack_bf16(o[tt][4 * r4] * p.scale, o[tt][4 * r4 + 1] * p.scale),
-                               pack_bf16(o[tt][4 * r4 + 2] * p.scale, o[tt][4 * r4 + 3] * p.scale)};
-            *(u32x2*)(strip + (32 * tt + l31) * kStrip + 16 * r4 + 8 * half) = two;
-          }
-        __builtin_amdgcn_wave_barrier();  // the strip is this wave's own: its LDS accesses stay in order
+        for (int r4 = 0; r4 < 4; ++r4)
+          *(u32x2*)(strip + l31 * kStrip + 16 * r4 + 8 * half) = u32x2{pack_bf16(o[4 * r4] * p.scale, o[4 * r4 + 1] * p.scale),
+                                                                       pack_bf16(o[4 * r4 + 2] * p.scale, o[4 * r4 + 3] * p.scale)};
+        __builtin_amdgcn_wave_barrier();
         char* out = (char*)p.out + (((int64_t)(g.t0 + c * kChunk) * p.Hq + h * p.group + gq) * p.Dv + c0 + 32 * w) * 2;
         const int piece = lane & 3, cols = p.Dv - c0 - 32 * w - 8 * piece;  // columns of the piece that exist
         for (int row = lane >> 2; row < n; row += 16) {
@@ -390,14 +378,17 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[d][r] = fmaf(S[d][r], l.y, S[d][r] * l.x);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < 2; ++ks) {
       const int m = 16 * ks + 8 * half;
-      const u32x2 x = column_operand<DV>(sV, m, vcol), y = column_operand<DV>(sV, m + 4, vcol);
+      if constexpr (!OUT) {
+        const u32x2 x = column_operand<DV>(tV, m, vcol), y = column_operand<DV>(tV, m + 4, vcol);
+        vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
+      }
       u32x4 hi, mid, lo;
-      split3(u32x4{x[0], x[1], y[0], y[1]}, *(const float4*)&left[m], *(const float4*)&left[m + 4], hi, mid, lo);
+      split3(vop[ks], *(const float4*)&left[m], *(const float4*)&left[m + 4], hi, mid, lo);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const u32x2 u = column_operand<DK>(sK, m, 32 * d + kcol), z = column_operand<DK>(sK, m + 4, 32 * d + kcol);
+        const u32x2 u = column_operand<DK>(tK, m, 32 * d + kcol), z = column_operand<DK>(tK, m + 4, 32 * d + kcol);
         const u32x4 kt = {u[0], u[1], z[0], z[1]};
         S[d] = mfma_bf16(kt, lo, S[d]);
         S[d] = mfma_bf16(kt, mid, S[d]);
@@ -420,20 +411,21 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
     }
 }
 
-template <int DK, int NW>
+template <int DK, int NW, bool VEC>
 void launch_bf16(hipStream_t stream, const DecayParams& p) {
   const int slices = (p.Dv + 32 * NW - 1) / (32 * NW), heads = p.Hkv * slices;
   if (p.slots > 0) {
-    hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), dim3(p.slots * heads), dim3(64 * NW), 0, stream, p);
+    hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false, VEC>), dim3(p.slots * heads), dim3(64 * NW), 0, stream, p);
     hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
   }
-  hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true>), dim3((p.first_ids + p.slots) * heads), dim3(64 * NW), 0, stream, p);
+  hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true, VEC>), dim3((p.first_ids + p.slots) * heads), dim3(64 * NW), 0, stream, p);
 }
 
 template <int DK>
 void launch_bf16_cols(hipStream_t stream, const DecayParams& p) {
-  if (p.Dv <= 64) launch_bf16<DK, 2>(stream, p);
-  else launch_bf16<DK, 4>(stream, p);
+  if (!p.vec) launch_bf16<DK, 4, false>(stream, p);
+  else if (p.Dv <= 64) launch_bf16<DK, 2, true>(stream, p);
+  else launch_bf16<DK, 4, true>(stream, p);
 }
 
 }  // namespace
