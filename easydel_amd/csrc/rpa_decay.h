@@ -54,10 +54,11 @@ __device__ __forceinline__ DecaySeq decay_seq(const DecayParams& p, int i) {
   return s;
 }
 
-// exp(g n) as an unevaluated sum of two floats: a factor that a long prompt applies hundreds of times must not carry its
-// own rounding along.  -inf (nothing kept) times 0 would be NaN, so g is held at a value whose exponential is 0.
+// exp(g n): -inf (nothing kept) times 0 would be NaN, so g is held at a value whose exponential is 0.  decay_power gives it as an
+// unevaluated sum of two floats: a factor that a long prompt applies hundreds of times must not carry its own rounding along.
+__device__ __forceinline__ double decay_exact(float g, int n) { return exp((double)(g < -1e30f ? -1e30f : g) * (double)n); }
 __device__ __forceinline__ float2 decay_power(float g, int n) {
-  const double e = exp((double)(g < -1e30f ? -1e30f : g) * (double)n);
+  const double e = decay_exact(g, n);
   const float hi = (float)e;
   return make_float2(hi, __builtin_isfinite(hi) ? (float)(e - (double)hi) : 0.f);
 }

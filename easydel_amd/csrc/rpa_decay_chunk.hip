@@ -154,36 +154,59 @@ __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(
 
 __device__ uint4 decay_zeros;  // 16 bytes of zeros: the source of what a tile holds beyond its rows and columns
 
-// Starts a tile of kChunk rows of WIDTH elements on its way into LDS; rows 0 .. n-1 of `cols` elements exist, `stride` elements
-// apart, the others become zeros.  VEC: direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's
-// vector-memory counter says so.  Otherwise rows at any address, element by element, complete at the next barrier.
+// A tile of kChunk rows of WIDTH elements on its way into LDS: rows 0 .. n-1 of `cols` elements exist, `stride` elements apart, the
+// others become zeros.  VEC: direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's vector-memory
+// counter says so; a whole tile takes its lanes' offsets from registers and its base from scalars.  Otherwise rows at any
+// address, element by element, complete at the next barrier.
 template <int WIDTH, int NT, bool VEC>
-__device__ __forceinline__ void start_tile(char* tile, const uint16_t* src, int64_t stride, int n, int cols) {
-  constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT;
+struct TileLoad {
+  static constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT;
   static_assert(N >= 1, "at least one piece a thread");
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    // wave w's instruction k fills bytes [(w N + k) 1024, + 1024) of the tile
-    const int piece = ((threadIdx.x >> 6) * N + k) * 64 + (threadIdx.x & 63), row = piece / PER_ROW;
-    const int c = ((piece % PER_ROW) ^ tile_key<WIDTH>(row)) * 8;
+  uint32_t at[VEC ? N : 1];
+  int64_t stride;
+  int cols;
+  // wave w's instruction k fills bytes [(w N + k) 1024, + 1024) of the tile
+  static __device__ __forceinline__ int piece(int k) { return ((threadIdx.x >> 6) * N + k) * 64 + (threadIdx.x & 63); }
+  static __device__ __forceinline__ int column(int k) { return ((piece(k) % PER_ROW) ^ tile_key<WIDTH>(piece(k) / PER_ROW)) * 8; }
+  __device__ __forceinline__ void init(int64_t stride_, int cols_) {
+    stride = stride_; cols = cols_;
     if constexpr (VEC) {
-      const void* at = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
-      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + ((threadIdx.x >> 6) * N + k) * 1024);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
-    } else {
-      uint64_t lo = 0, hi = 0;
-      if (row < n) {
-        const uint16_t* at = src + row * stride + c;
-#pragma unroll 1
-        for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
-          hi = (hi << 16) | (lo >> 48);
-          lo = (lo << 16) | at[x];
-        }
-      }
-      *(u32x4*)(tile + piece * 16) = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+#pragma unroll
+      for (int k = 0; k < N; ++k) at[k] = ((uint32_t)(piece(k) / PER_ROW) * (uint32_t)stride + column(k)) * 2;  // 32 rows span less than 2^31 bytes
     }
   }
-}
+  __device__ __forceinline__ void start(char* tile, const uint16_t* src, int n) const {
+    if constexpr (VEC) {
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + (threadIdx.x >> 6) * N * 1024);
+      if (n >= kChunk && cols >= WIDTH) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) dma16(to + k * 1024, at[k], src);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int row = piece(k) / PER_ROW, c = column(k);
+          const void* from = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + k * 1024), "v"(from) : "memory");
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int row = piece(k) / PER_ROW, c = column(k);
+        uint64_t lo = 0, hi = 0;
+        if (row < n) {
+          const uint16_t* from = src + row * stride + c;
+#pragma unroll 1
+          for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
+            hi = (hi << 16) | (lo >> 48);
+            lo = (lo << 16) | from[x];
+          }
+        }
+        *(u32x4*)(tile + piece(k) * 16) = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      }
+    }
+  }
+};
 
 // Eight decayed values as three bf16 operands whose sum is the float32 value.
 __device__ __forceinline__ void split3(u32x4 v, const float4& w0, const float4& w1, u32x4& hi, u32x4& mid, u32x4& lo) {
@@ -216,25 +239,31 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
   __shared__ __align__(16) char sO[OUT ? NW * kChunk * kStrip : 16];
   __shared__ __align__(16) float pw[kChunk + 4];  // l^0 .. l^C
   __shared__ __align__(16) float left[kChunk];    // l^(n-1-m) for the n tokens m of a chunk, 0 behind them
-  __shared__ float2 whole[2];                     // l^n of a full chunk and of the last one, as two floats
 
   const int slices = (p.Dv + DV - 1) / DV, heads = p.Hkv * slices;
   const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
   Segment g;
   if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, l31 = lane & 31;
-  const int chunks = (g.n + kChunk - 1) / kChunk, tail = g.n - (chunks - 1) * kChunk;
+  const int chunks = (g.n + kChunk - 1) / kChunk;
   const uint16_t* q = (const uint16_t*)p.q + (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk;
   const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
   const uint16_t* v = (const uint16_t*)p.v + (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
   const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
-  start_tile<DK, NT, VEC>(sK[0], k, p.k_stride, g.n, p.Dk);
-  start_tile<DV, NT, VEC>(sV[0], v, p.v_stride, g.n, vcols);
-  if constexpr (OUT) start_tile<DK, NT, VEC>(sQ[0], q, p.q_stride, g.n, p.Dk);
+  TileLoad<DK, NT, VEC> lq, lk;
+  TileLoad<DV, NT, VEC> lv;
+  lk.init(p.k_stride, p.Dk);
+  lv.init(p.v_stride, vcols);
+  const int64_t first = OUT ? 0 : (int64_t)(chunks - 1) * kChunk;
+  lk.start(sK[0], k + first * p.k_stride, g.n);
+  lv.start(sV[0], v + first * p.v_stride, g.n);
+  if constexpr (OUT) {
+    lq.init(p.q_stride, p.Dk);
+    lq.start(sQ[0], q, g.n);
+  }
 
   const float rate = p.log_decay[h];
   if (tid <= kChunk) pw[tid] = decay_power(rate, tid).x;
-  else if (tid < kChunk + 3) whole[tid - kChunk - 1] = decay_power(rate, tid == kChunk + 1 ? kChunk : tail);
   if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_power(rate, kChunk - 1 - (tid - 64)).x;
   if constexpr (OUT) {
     if (tid < 64) *(u32x4*)(sP + (tid & 15) * kStrip + 32 + (tid >> 4 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};  // the tile of masked scores alone
@@ -258,12 +287,19 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
       }
   }
 
+  // The state is multiplied by l^C once a chunk: each factor is rounded so that the product of all of them so far stays within a
+  // rounding of the true power (`off`: how far it is, relatively), however long the segment.
+  const double full_power = decay_exact(rate, kChunk);
+  const double tail_power = decay_exact(rate, g.n - (chunks - 1) * kChunk);
+  const double per = full_power > 0.0 ? 1.0 / full_power : 0.0;
+  double off = 0.0, over = 1.0;
+
   // this lane's share of the transposing loads
   const int vcol = 32 * w + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const int kcol = 16 * ((lane >> 4) & 1) + 4 * (((lane & 1) << 1) | ((lane >> 1) & 1));
 
   for (int c = 0; c < chunks; ++c) {
-    const int n = min(g.n - c * kChunk, kChunk);
+    const int n = OUT ? min(g.n - c * kChunk, kChunk) : kChunk;
     const char *tK = sK[c & 1], *tV = sV[c & 1];
     u32x4 vop[2];
     for (int gq = 0; gq < groups; ++gq) {
@@ -274,17 +310,14 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
       const bool on = gq == groups - 1;  // the next step is another chunk's
       const int cn = c + (on ? 1 : 0);
       if (cn < chunks) {
-        const int64_t ahead = (int64_t)cn * kChunk;
-        if constexpr (OUT) start_tile<DK, NT, VEC>(sQ[(step + 1) & 1], q + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), p.q_stride, g.n - cn * kChunk, p.Dk);
+        const int64_t ahead = (int64_t)(OUT ? cn : chunks - 1 - cn) * kChunk;
+        if constexpr (OUT) lq.start(sQ[(step + 1) & 1], q + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), g.n - cn * kChunk);
         if (on) {
-          start_tile<DK, NT, VEC>(sK[cn & 1], k + ahead * p.k_stride, p.k_stride, g.n - cn * kChunk, p.Dk);
-          start_tile<DV, NT, VEC>(sV[cn & 1], v + ahead * p.v_stride, p.v_stride, g.n - cn * kChunk, vcols);
+          lk.start(sK[cn & 1], k + ahead * p.k_stride, OUT ? g.n - cn * kChunk : kChunk);
+          lv.start(sV[cn & 1], v + ahead * p.v_stride, OUT ? g.n - cn * kChunk : kChunk);
         }
       }
-      if (n < kChunk && gq == 0) {  // the last chunk alone
-        if (tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;
-        if constexpr (!OUT) __syncthreads();
-      }
+      if (n < kChunk && gq == 0 && tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;  // the last chunk alone
       if constexpr (OUT) {
         const char* tQ = sQ[step & 1];
         // scores, decayed and masked: tile (keys 16 a.., queries 16 b..) of S^T
@@ -372,11 +405,19 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
       }
     }
     if (OUT && c == chunks - 1 && (!g.last || g.out < 0)) break;  // nobody reads the state behind this chunk
-    const float2 l = whole[n < kChunk ? 1 : 0];
+    // OUT: the state is decayed over the chunk.  Otherwise it starts from zero, the chunks come last to first (all are whole) and
+    // their tokens enter with their decay to the end of the segment, which leaves the state alone.
+    const float behind = (float)over;
+    over *= full_power;
+    if constexpr (OUT) {
+      const double exact = n < kChunk ? tail_power : full_power;
+      const float l = (float)(exact * (1.0 - off));
+      off += ((double)l - exact) * per;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[d][r] = fmaf(S[d][r], l.y, S[d][r] * l.x);
+        for (int r = 0; r < 16; ++r) S[d][r] *= l;
+    }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int m = 16 * ks + 8 * half;
@@ -385,7 +426,12 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
         vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
       }
       u32x4 hi, mid, lo;
-      split3(vop[ks], *(const float4*)&left[m], *(const float4*)&left[m + 4], hi, mid, lo);
+      float4 w0 = *(const float4*)&left[m], w1 = *(const float4*)&left[m + 4];
+      if constexpr (!OUT) {
+        w0.x *= behind; w0.y *= behind; w0.z *= behind; w0.w *= behind;
+        w1.x *= behind; w1.y *= behind; w1.z *= behind; w1.w *= behind;
+      }
+      split3(vop[ks], w0, w1, hi, mid, lo);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const u32x2 u = column_operand<DK>(tK, m, 32 * d + kcol), z = column_operand<DK>(tK, m + 4, 32 * d + kcol);
