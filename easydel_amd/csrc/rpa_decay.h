@@ -57,6 +57,8 @@ __device__ __forceinline__ DecaySeq decay_seq(const DecayParams& p, int i) {
 // exp(g n): -inf (nothing kept) times 0 would be NaN, so g is held at a value whose exponential is 0.  decay_power gives it as an
 // unevaluated sum of two floats: a factor that a long prompt applies hundreds of times must not carry its own rounding along.
 __device__ __forceinline__ double decay_exact(float g, int n) { return exp((double)(g < -1e30f ? -1e30f : g) * (double)n); }
+// ... in float32, off by |g n| 2^-24 at most where that counts: for a factor applied once.
+__device__ __forceinline__ float decay_float(float g, int n) { return expf((g < -1e30f ? -1e30f : g) * (float)n); }
 __device__ __forceinline__ float2 decay_power(float g, int n) {
   const double e = decay_exact(g, n);
   const float hi = (float)e;

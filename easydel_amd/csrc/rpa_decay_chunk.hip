@@ -18,8 +18,6 @@ namespace rpa {
 
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 struct Segment {
   int j, t0, n;      // segment of its sequence, first token, tokens
   int in, out;       // slots of the sequence
@@ -105,20 +103,21 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
 }
 
 // ---- bfloat16: matrix instructions on bf16 operands ---------------------------------------------------------
-// Chunks of 32 tokens.  Wave w owns 32 columns of the state and of the output: its part of S stays in accumulators for the whole
-// segment, as 32 x 32 tiles whose lane half h and register r hold key 32 d + 16 (r / 8) + 8 h + r % 8.  In that order eight
-// registers, rounded to bf16, are one operand of the product with the queries as they lie in memory; the order comes for free,
-// since the rows of K^T can be read in any order of four.
-//   scores   S^T = K Q^T, three of the four 16 x 16 tiles, shared out over the waves, through LDS as bf16
+// Chunks of 32 tokens, 16 x 16 tiles (32 k-values an instruction).  Wave w owns 16 columns of the state and of the output: its part
+// of S stays in accumulators for the whole segment.  Lane (i, g) = (lane & 15, lane / 16) holds column i; register j of tile d
+// holds key 32 (d / 2) + 8 g + 4 (d & 1) + j, so that two tiles, rounded to bf16, are one operand of the product with the queries
+// as they lie in memory.  The order comes for free: the rows of K^T can be read in any order of four.
+//   scores   S^T = K Q^T, three of the four tiles, one a wave, through LDS as bf16
 //   output   O^T = S0^T Q^T, columns scaled by l^(n+1) in float32, then + V^T P^T
 //   state    l^n S + K^T (l^(n-1-m) V): the decayed values are float32, so they enter as the sum of three bf16 numbers
 //            (24 bits); the state keeps float32 accuracy.
 // Rounded to bf16 are the scores and, for the product with the queries only, the state: what they add to an output is rounded
-// to bf16 as well.  The tiles of the next chunk are on their way into LDS (direct loads, two buffers) while this one is worked on;
-// registers hold no tile in flight, so two workgroups share a CU and fill each other's waits.
+// to bf16 as well.  The tiles of the next chunk are on their way into LDS (direct loads, two buffers) while this one is worked on.
+// What a chunk costs is mostly the latency of its chain (tiles, scores, barrier, products, store); sixteen waves a CU with 16
+// columns each hide it better than eight with 32.
 
 constexpr int kChunk = 32;
-constexpr int kStrip = 80;  // bytes of a row of 32 bf16 values in LDS, spread over the banks
+constexpr int kScoreRow = 80;  // bytes of a row of 32 bf16 scores in LDS, spread over the banks
 
 // 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key: eight consecutive rows read at one chunk, and four
 // rows read at a pair of chunks by the transposing loads, fall on distinct banks.
@@ -131,23 +130,57 @@ __device__ __forceinline__ int tile_key(int row) {
 typedef __attribute__((address_space(3))) const char lds_char;
 __device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
-template <int WIDTH>
-__device__ __forceinline__ u32x4 row_operand(const char* tile, int row, int chunk) {
-  return *(const u32x4*)(tile + row * WIDTH * 2 + ((chunk ^ tile_key<WIDTH>(row)) << 4));
+__device__ __forceinline__ u32x4 lds_read(uint32_t at) { return *(__attribute__((address_space(3))) const u32x4*)(uintptr_t)at; }
+__device__ __forceinline__ u32x2 lds_read_columns(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
 }
 
-// Four rows from `row` on of sixteen columns, one column a lane (of each group of sixteen): the lane supplies the address of row
-// row + (lane & 15) / 4 and of the four columns `mine` on that lanes 4 (lane & 3) .. + 3 are to hold.
+// Where a lane reads a tile of rows of WIDTH elements.  The XOR of a chunk number with the row's key splits into the lane's part,
+// held in a few registers, and parts that are the same for all lanes and become the reads' immediate offsets.
 template <int WIDTH>
-__device__ __forceinline__ u32x2 column_operand(const char* tile, int row, int mine) {
-  const int r = row + ((threadIdx.x & 15) >> 2);
-  const char* a = tile + r * WIDTH * 2 + (((mine >> 3) ^ tile_key<WIDTH>(r)) << 4) + ((mine & 7) << 1);
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds_address(a)));
-}
+struct TileRows {  // row i (of sixteen, more a constant further on), eight elements from 32 ks + 8 g on
+  static constexpr int N = WIDTH >= 128 ? 4 : WIDTH / 32;
+  uint32_t at[N];
+  __device__ __forceinline__ void init(int i16, int g4) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) at[k] = i16 * WIDTH * 2 + (((4 * k + g4) ^ tile_key<WIDTH>(i16)) << 4);
+  }
+  __device__ __forceinline__ u32x4 read(uint32_t tile, int row16, int ks) const { return lds_read(tile + at[ks % N] + (ks / N) * (N * 64) + row16 * 16 * WIDTH * 2); }
+};
+template <int WIDTH>
+struct TileColumns {  // rows 8 g .. 8 g + 7 of the columns that the transposing reads hand out, four of them from this lane's address on
+  uint32_t at[2];  // the first four rows' and the last four rows'
+  // `column`: a multiple of 4 of this lane's own
+  __device__ __forceinline__ void init(int g4, int lane, int column) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int row = 8 * g4 + ((lane & 15) >> 2) + 4 * y;
+      at[y] = row * WIDTH * 2 + (((column >> 3) ^ tile_key<WIDTH>(row)) << 4) + ((column & 7) << 1);
+    }
+  }
+  __device__ __forceinline__ u32x4 read(uint32_t tile) const {
+    const u32x2 x = lds_read_columns(tile + at[0]), y = lds_read_columns(tile + at[1]);
+    return u32x4{x[0], x[1], y[0], y[1]};
+  }
+};
+template <int WIDTH>
+struct TileKeys {  // the same for columns 32 s + 8 (lane & 3) + 4 odd: chunk 4 s + (lane & 3), whose lane part is below 8 (4 for narrow rows)
+  uint32_t at[2];  // at[x]: the chunk's lane part, bit 2 flipped for odd s where the key reaches it
+  __device__ __forceinline__ void init(int g4, int lane) {
+    const int row = 8 * g4 + ((lane & 15) >> 2), part = (lane & 3) ^ tile_key<WIDTH>(row);
+    at[0] = row * WIDTH * 2 + (part << 4);
+    at[1] = row * WIDTH * 2 + ((part ^ 4) << 4);
+  }
+  __device__ __forceinline__ u32x4 read(uint32_t tile, int s, int odd) const {
+    // the key of the row four further on differs in bit 3 of the chunk (wide rows) or bit 2 (narrow ones)
+    const int sx = s, sy = WIDTH >= 128 ? s ^ 2 : s ^ 1;
+    const u32x2 x = lds_read_columns(tile + (WIDTH >= 128 ? at[sx & 1] + (sx >> 1) * 128 : at[sx & 1]) + 8 * odd);
+    const u32x2 y = lds_read_columns(tile + (WIDTH >= 128 ? at[sy & 1] + (sy >> 1) * 128 : at[sy & 1]) + 8 * odd + 4 * WIDTH * 2);
+    return u32x4{x[0], x[1], y[0], y[1]};
+  }
+};
 
-__device__ __forceinline__ f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) { return HalfOf<RPA_BF16>::mfma32(a, b, c); }
 
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -160,8 +193,7 @@ __device__ uint4 decay_zeros;  // 16 bytes of zeros: the source of what a tile h
 // address, element by element, complete at the next barrier.
 template <int WIDTH, int NT, bool VEC>
 struct TileLoad {
-  static constexpr int PER_ROW = WIDTH / 8, N = kChunk * PER_ROW / NT;
-  static_assert(N >= 1, "at least one piece a thread");
+  static constexpr int PER_ROW = WIDTH / 8, PIECES = kChunk * PER_ROW, N = PIECES >= NT ? PIECES / NT : 1;  // fewer pieces than threads: the first waves'
   uint32_t at[VEC ? N : 1];
   int64_t stride;
   int cols;
@@ -176,6 +208,7 @@ struct TileLoad {
     }
   }
   __device__ __forceinline__ void start(char* tile, const uint16_t* src, int n) const {
+    if (PIECES < NT && (int)threadIdx.x >= PIECES) return;
     if constexpr (VEC) {
       const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + (threadIdx.x >> 6) * N * 1024);
       if (n >= kChunk && cols >= WIDTH) {
@@ -229,14 +262,13 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 }
 
 template <int DK, int NW, bool OUT, bool VEC>
-__global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
-  constexpr int NT = 64 * NW, DV = 32 * NW, ND = DK / 32;
+__global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
+  constexpr int NT = 64 * NW, DV = 16 * NW, ND = DK / 16;
   constexpr int KB = kChunk * DK * 2, VB = kChunk * DV * 2;
   __shared__ __align__(1024) char sK[2][KB];
   __shared__ __align__(1024) char sV[2][VB];
   __shared__ __align__(1024) char sQ[OUT ? 2 : 1][OUT ? KB : 16];
-  __shared__ __align__(16) char sP[OUT ? kChunk * kStrip : 16];
-  __shared__ __align__(16) char sO[OUT ? NW * kChunk * kStrip : 16];
+  __shared__ __align__(16) char sP[OUT ? kChunk * kScoreRow : 16];
   __shared__ __align__(16) float pw[kChunk + 4];  // l^0 .. l^C
   __shared__ __align__(16) float left[kChunk];    // l^(n-1-m) for the n tokens m of a chunk, 0 behind them
 
@@ -244,7 +276,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
   const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
   Segment g;
   if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, l31 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, i16 = lane & 15, g4 = lane >> 4;
   const int chunks = (g.n + kChunk - 1) / kChunk;
   const uint16_t* q = (const uint16_t*)p.q + (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk;
   const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
@@ -262,50 +294,56 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
     lq.start(sQ[0], q, g.n);
   }
 
-  const float rate = p.log_decay[h];
-  if (tid <= kChunk) pw[tid] = decay_power(rate, tid).x;
-  if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_power(rate, kChunk - 1 - (tid - 64)).x;
-  if constexpr (OUT) {
-    if (tid < 64) *(u32x4*)(sP + (tid & 15) * kStrip + 32 + (tid >> 4 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};  // the tile of masked scores alone
-  }
-
-  const int col = c0 + 32 * w + l31;
+  const int col = c0 + 16 * w + i16;
   const bool mine = col < p.Dv;
-  f32x16 S[ND];
+  f32x4 S[ND];
   const float* from = OUT ? state_ahead(p, g, h) : nullptr;
 #pragma unroll
-  for (int d = 0; d < ND; ++d) S[d] = f32x16{};
+  for (int d = 0; d < ND; ++d) S[d] = f32x4{};
   if (from != nullptr) {
     const float* at = from + (mine ? col : 0);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 32 * d + 16 * (r >> 3) + 8 * half + (r & 7);
+      for (int j = 0; j < 4; ++j) {
+        const int key = 32 * (d >> 1) + 8 * g4 + 4 * (d & 1) + j;
         const float x = at[min(key, p.Dk - 1) * p.Dv];  // unconditional loads, all in flight at once
-        S[d][r] = mine && key < p.Dk ? x : 0.f;
+        S[d][j] = mine && key < p.Dk ? x : 0.f;
       }
   }
+  // The state is multiplied by l^C = full.x + full.y once a chunk: each factor is rounded so that the product of all of them so
+  // far stays within a rounding of the true power (`off`: how far it is, relatively), however long the segment.
+  const float rate = p.log_decay[h];
+  const float2 full = decay_power(rate, kChunk);
+  const float per = full.x > 0.f ? 1.f / full.x : 0.f;
+  float off = 0.f;
+  double over = 1.0;
+  if (tid <= kChunk) pw[tid] = decay_float(rate, tid);
+  if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_float(rate, kChunk - 1 - (tid - 64));
+  if constexpr (OUT) {
+    if (tid >= 128 && tid < 160) *(u32x4*)(sP + (tid & 15) * kScoreRow + 32 + (tid >> 4 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};  // the tile of masked scores alone
+  }
 
-  // The state is multiplied by l^C once a chunk: each factor is rounded so that the product of all of them so far stays within a
-  // rounding of the true power (`off`: how far it is, relatively), however long the segment.
-  const double full_power = decay_exact(rate, kChunk);
-  const double tail_power = decay_exact(rate, g.n - (chunks - 1) * kChunk);
-  const double per = full_power > 0.0 ? 1.0 / full_power : 0.0;
-  double off = 0.0, over = 1.0;
-
-  // this lane's share of the transposing loads
-  const int vcol = 32 * w + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const int kcol = 16 * ((lane >> 4) & 1) + 4 * (((lane & 1) << 1) | ((lane >> 1) & 1));
-
+  TileRows<DK> rows;
+  TileKeys<DK> keys;
+  TileColumns<DV> columns;
+  rows.init(i16, g4);
+  keys.init(g4, lane);
+  columns.init(g4, lane, 16 * w + 4 * (lane & 3));
+  const uint32_t aK = lds_address(sK[0]), aV = lds_address(sV[0]), aQ = lds_address(sQ[0]), aP = lds_address(sP);
+  const bool whole = OUT && c0 + 16 * w + 16 <= p.Dv;
   for (int c = 0; c < chunks; ++c) {
     const int n = OUT ? min(g.n - c * kChunk, kChunk) : kChunk;
-    const char *tK = sK[c & 1], *tV = sV[c & 1];
-    u32x4 vop[2];
+    const uint32_t tK = aK + (c & 1) * KB, tV = aV + (c & 1) * VB;
+    u32x4 vop;  // tokens 8 g .. 8 g + 7 of column i
     for (int gq = 0; gq < groups; ++gq) {
       const int step = c * groups + gq;
-      // this step's tiles have arrived (so have the output rows of the step before), and the other buffers have been read
-      if constexpr (VEC) wait_loads<0>();
+      // this step's tiles have arrived, and the other buffers have been read.  Behind the tiles' loads this wave issued the two
+      // stores of the step before where it holds 16 columns (`whole`): they need not be waited for.
+      if constexpr (VEC) {
+        if (whole && step > 0) wait_loads<2>();
+        else wait_loads<0>();
+      }
       __syncthreads();
       const bool on = gq == groups - 1;  // the next step is another chunk's
       const int cn = c + (on ? 1 : 0);
@@ -318,18 +356,16 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
         }
       }
       if (n < kChunk && gq == 0 && tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;  // the last chunk alone
+      vop = columns.read(tV);
       if constexpr (OUT) {
-        const char* tQ = sQ[step & 1];
+        const uint32_t tQ = aQ + (step & 1) * KB;
         // scores, decayed and masked: tile (keys 16 a.., queries 16 b..) of S^T
-        const int i16 = lane & 15, g4 = lane >> 4;
-#pragma unroll
-        for (int tile = 0; tile < 3; ++tile) {
-          if (tile % NW != w) continue;
-          const int a = tile == 1 ? 1 : 0, b = tile == 0 ? 0 : 1;
+        if (w < 3) {
+          const int a = w == 1 ? 1 : 0, b = w == 0 ? 0 : 1;
           f32x4 acc = {};
 #pragma unroll
           for (int ks = 0; ks < DK / 32; ++ks)
-            acc = HalfOf<RPA_BF16>::mfma32(row_operand<DK>(tK, 16 * a + i16, 4 * ks + g4), row_operand<DK>(tQ, 16 * b + i16, 4 * ks + g4), acc);
+            acc = mfma_bf16(rows.read(tK + a * 16 * DK * 2, 0, ks), rows.read(tQ + b * 16 * DK * 2, 0, ks), acc);
           const int t = 16 * b + i16, s0 = 16 * a + 4 * g4;
           float f[4];
 #pragma unroll
@@ -337,129 +373,107 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 2 : 1) void decay_chunk_bf16_k
             const int gap = t - s0 - e;
             f[e] = gap >= 0 ? acc[e] * pw[max(gap, 0)] : 0.f;  // chosen, not multiplied: masked scores may be infinite
           }
-          *(u32x2*)(sP + t * kStrip + s0 * 2) = u32x2{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
+          *(u32x2*)(sP + t * kScoreRow + s0 * 2) = u32x2{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
         }
-        __syncthreads();
-        // O^T of this wave's columns: lane = token, registers = columns 8 (r / 4) + 4 half + r % 4
-        f32x16 o = {};
+        // O^T of this wave's columns: lane i = token, registers = columns 4 g + j; its product with the state needs no scores
+        f32x4 o[2] = {};
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int s = 0; s < ND / 2; ++s) {
+          const u32x4 st = {pack_bf16(S[2 * s][0], S[2 * s][1]), pack_bf16(S[2 * s][2], S[2 * s][3]),
+                            pack_bf16(S[2 * s + 1][0], S[2 * s + 1][1]), pack_bf16(S[2 * s + 1][2], S[2 * s + 1][3])};
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const u32x4 s = {pack_bf16(S[d][8 * x], S[d][8 * x + 1]), pack_bf16(S[d][8 * x + 2], S[d][8 * x + 3]),
-                             pack_bf16(S[d][8 * x + 4], S[d][8 * x + 5]), pack_bf16(S[d][8 * x + 6], S[d][8 * x + 7])};
-            o = mfma_bf16(s, row_operand<DK>(tQ, l31, 4 * d + 2 * x + half), o);
-          }
-        const float ahead_of = pw[l31 + 1];
+          for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(st, rows.read(tQ, tt, s), o[tt]);
+        }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[r] *= ahead_of;
+        for (int tt = 0; tt < 2; ++tt) o[tt] *= pw[16 * tt + i16 + 1];
         // A value that is not finite would meet the zeros of the masked scores as well, and 0 x Inf is NaN: such values stay out of
         // the product, and the rows that see one become NaN by hand.
-        uint32_t full = 0;
+        uint32_t ones = 0;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const u32x2 x = column_operand<DV>(tV, 16 * ks + 8 * half, vcol), y = column_operand<DV>(tV, 16 * ks + 8 * half + 4, vcol);
-          vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) full |= (vop[ks][e] & 0x7f807f80u) + 0x00800080u;  // bit 15 or 31: an exponent of all ones
-        }
-        const bool odd = __any((full & 0x80008000u) != 0);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          u32x4 vo = vop[ks];
-          if (odd) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vo[e] = finite_halves(vo[e]);
-          }
-          o = mfma_bf16(vo, *(const u32x4*)(sP + l31 * kStrip + (2 * ks + half) * 16), o);
-        }
+        for (int e = 0; e < 4; ++e) ones |= (vop[e] & 0x7f807f80u) + 0x00800080u;  // bit 15 or 31: an exponent of all ones
+        const bool odd = __any((ones & 0x80008000u) != 0);
+        u32x4 vo = vop;
         if (odd) {
-          const int at = 32 * w + l31;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vo[e] = finite_halves(vo[e]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(vo, lds_read(aP + (16 * tt + i16) * kScoreRow + g4 * 16), o[tt]);
+        if (odd) {
+          const int at = 16 * w + i16;
           int bad = 0;
           for (; bad < n; ++bad) {
-            const uint16_t bits = *(const uint16_t*)(tV + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
+            const uint16_t bits = *(const uint16_t*)(sV[c & 1] + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
             if ((bits & 0x7f80) == 0x7f80) break;
           }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int first = __shfl(bad, 8 * (r >> 2) + 4 * half + (r & 3));
-            o[r] = l31 >= first ? __builtin_nanf("") : o[r];
+          for (int j = 0; j < 4; ++j) {
+            const int first_bad = __shfl(bad, 4 * g4 + j);
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) o[tt][j] = 16 * tt + i16 >= first_bad ? __builtin_nanf("") : o[tt][j];
           }
         }
-        // through this wave's own strip of LDS (whose accesses stay in order) to whole rows of 32 columns
-        char* strip = sO + w * kChunk * kStrip;
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4)
-          *(u32x2*)(strip + l31 * kStrip + 16 * r4 + 8 * half) = u32x2{pack_bf16(o[4 * r4] * p.scale, o[4 * r4 + 1] * p.scale),
-                                                                       pack_bf16(o[4 * r4 + 2] * p.scale, o[4 * r4 + 3] * p.scale)};
-        __builtin_amdgcn_wave_barrier();
-        char* out = (char*)p.out + (((int64_t)(g.t0 + c * kChunk) * p.Hq + h * p.group + gq) * p.Dv + c0 + 32 * w) * 2;
-        const int piece = lane & 3, cols = p.Dv - c0 - 32 * w - 8 * piece;  // columns of the piece that exist
-        for (int row = lane >> 2; row < n; row += 16) {
-          const u32x4 v8 = *(const u32x4*)(strip + row * kStrip + 16 * piece);
-          char* to = out + (int64_t)row * p.Hq * p.Dv * 2 + 16 * piece;
-          if (cols >= 8 && (p.Dv & 7) == 0) *(u32x4*)to = v8;
-          else if (cols >= 4) { *(u32x2*)to = u32x2{v8[0], v8[1]}; if (cols >= 8) *(u32x2*)(to + 8) = u32x2{v8[2], v8[3]}; }
+        // four columns a lane, 32 bytes of a row a wave
+        char* out = (char*)p.out + (((int64_t)(g.t0 + c * kChunk) * p.Hq + h * p.group + gq) * p.Dv + c0 + 16 * w) * 2;
+        const uint32_t at = (uint32_t)(i16 * p.Hq * p.Dv + 4 * g4) * 2, half = (uint32_t)(16 * p.Hq * p.Dv) * 2;
+        const u32x2 lo = {pack_bf16(o[0][0] * p.scale, o[0][1] * p.scale), pack_bf16(o[0][2] * p.scale, o[0][3] * p.scale)};
+        const u32x2 hi = {pack_bf16(o[1][0] * p.scale, o[1][1] * p.scale), pack_bf16(o[1][2] * p.scale, o[1][3] * p.scale)};
+        if (whole && n == kChunk) {
+          *(u32x2*)(out + at) = lo;
+          *(u32x2*)(out + half + at) = hi;
+        } else if (c0 + 16 * w + 4 * g4 < p.Dv) {
+          if (i16 < n) *(u32x2*)(out + at) = lo;
+          if (i16 + 16 < n) *(u32x2*)(out + half + at) = hi;
         }
-        __builtin_amdgcn_wave_barrier();
       }
     }
     if (OUT && c == chunks - 1 && (!g.last || g.out < 0)) break;  // nobody reads the state behind this chunk
     // OUT: the state is decayed over the chunk.  Otherwise it starts from zero, the chunks come last to first (all are whole) and
     // their tokens enter with their decay to the end of the segment, which leaves the state alone.
-    const float behind = (float)over;
-    over *= full_power;
+    float behind = 1.f;
     if constexpr (OUT) {
-      const double exact = n < kChunk ? tail_power : full_power;
-      const float l = (float)(exact * (1.0 - off));
-      off += ((double)l - exact) * per;
+      float l = n < kChunk ? pw[n] : full.x + (full.y - full.x * off);
+      off += ((l - full.x) - full.y) * per;
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) S[d][r] *= l;
+      for (int d = 0; d < ND; ++d) S[d] *= l;
+    } else {
+      behind = (float)over;
+      over *= (double)full.x + (double)full.y;
     }
+    float4 w0 = *(const float4*)&left[8 * g4], w1 = *(const float4*)&left[8 * g4 + 4];
+    if constexpr (!OUT) {
+      w0.x *= behind; w0.y *= behind; w0.z *= behind; w0.w *= behind;
+      w1.x *= behind; w1.y *= behind; w1.z *= behind; w1.w *= behind;
+    }
+    u32x4 hi, mid, lo;
+    split3(vop, w0, w1, hi, mid, lo);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int m = 16 * ks + 8 * half;
-      if constexpr (!OUT) {
-        const u32x2 x = column_operand<DV>(tV, m, vcol), y = column_operand<DV>(tV, m + 4, vcol);
-        vop[ks] = u32x4{x[0], x[1], y[0], y[1]};
-      }
-      u32x4 hi, mid, lo;
-      float4 w0 = *(const float4*)&left[m], w1 = *(const float4*)&left[m + 4];
-      if constexpr (!OUT) {
-        w0.x *= behind; w0.y *= behind; w0.z *= behind; w0.w *= behind;
-        w1.x *= behind; w1.y *= behind; w1.z *= behind; w1.w *= behind;
-      }
-      split3(vop[ks], w0, w1, hi, mid, lo);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const u32x2 u = column_operand<DK>(tK, m, 32 * d + kcol), z = column_operand<DK>(tK, m + 4, 32 * d + kcol);
-        const u32x4 kt = {u[0], u[1], z[0], z[1]};
-        S[d] = mfma_bf16(kt, lo, S[d]);
-        S[d] = mfma_bf16(kt, mid, S[d]);
-        S[d] = mfma_bf16(kt, hi, S[d]);
-      }
+    for (int d = 0; d < ND; ++d) {
+      const u32x4 kt = keys.read(tK, d >> 1, d & 1);
+      S[d] = mfma_bf16(kt, lo, S[d]);
+      S[d] = mfma_bf16(kt, mid, S[d]);
+      S[d] = mfma_bf16(kt, hi, S[d]);
     }
   }
   if (OUT && (!g.last || g.out < 0)) return;
   float* to = OUT ? p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv : scratch_state(p, g.base + g.j, h);
-  int back = 8 * half;
+  int back = 8 * g4;
   asm volatile("" : "+v"(back));  // the addresses and masks are not those of the beginning, kept through the loop
   if (!mine) return;
   float* at = to + back * p.Dv + col;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int key = 32 * d + 16 * (r >> 3) + (r & 7);
-      if (key + back < p.Dk) at[key * p.Dv] = S[d][r];
+    for (int j = 0; j < 4; ++j) {
+      const int key = 32 * (d >> 1) + 4 * (d & 1) + j;
+      if (key + back < p.Dk) at[key * p.Dv] = S[d][j];
     }
 }
 
 template <int DK, int NW, bool VEC>
 void launch_bf16(hipStream_t stream, const DecayParams& p) {
-  const int slices = (p.Dv + 32 * NW - 1) / (32 * NW), heads = p.Hkv * slices;
+  const int slices = (p.Dv + 16 * NW - 1) / (16 * NW), heads = p.Hkv * slices;
   if (p.slots > 0) {
     hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false, VEC>), dim3(p.slots * heads), dim3(64 * NW), 0, stream, p);
     hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
@@ -469,9 +483,9 @@ void launch_bf16(hipStream_t stream, const DecayParams& p) {
 
 template <int DK>
 void launch_bf16_cols(hipStream_t stream, const DecayParams& p) {
-  if (!p.vec) launch_bf16<DK, 4, false>(stream, p);
-  else if (p.Dv <= 64) launch_bf16<DK, 2, true>(stream, p);
-  else launch_bf16<DK, 4, true>(stream, p);
+  if (!p.vec) launch_bf16<DK, 8, false>(stream, p);
+  else if (p.Dv <= 64) launch_bf16<DK, 4, true>(stream, p);
+  else launch_bf16<DK, 8, true>(stream, p);
 }
 
 }  // namespace
