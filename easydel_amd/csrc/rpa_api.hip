@@ -944,10 +944,8 @@ static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayPara
 
 size_t rpa_decay_attention_workspace_bytes(int T, int S, int Hq, int Hkv, int Dk, int Dv, int dtype) {
   if (T <= rpa::kDecayRows || S <= 0 || Hq <= 0 || Hkv <= 0 || Dk <= 0 || Dv <= 0) return 0;
+  (void)dtype;
   rpa::DecayParams p;
-  memset(&p, 0, sizeof(p));
-  p.dtype = dtype;
-  if (!rpa::decay_chunk_supported(p)) return 0;
   size_t scratch;
   decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
   return scratch;
@@ -989,7 +987,7 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   hipStream_t s = (hipStream_t)stream;
   // (rows that lie 2^23 elements apart would pass the chunked form's 32-bit offsets in a chunk: the recurrent form takes them)
   const bool near = std::max(query_stride, std::max(key_stride, value_stride)) < ((int64_t)1 << 23);
-  if (T > rpa::kDecayRows && near && rpa::decay_chunk_supported(p)) {
+  if (T > rpa::kDecayRows && near) {
     size_t scratch;
     decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
     p.rows = rpa::kDecayRows;

@@ -65,7 +65,6 @@ __device__ __forceinline__ float2 decay_power(float g, int n) {
   return make_float2(hi, __builtin_isfinite(hi) ? (float)(e - (double)hi) : 0.f);
 }
 
-bool decay_chunk_supported(const DecayParams& p);
 int launch_decay_chunk(hipStream_t stream, const DecayParams& p);
 int launch_decay_recurrent(hipStream_t stream, const DecayParams& p);
 

@@ -119,12 +119,13 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
 constexpr int kChunk = 32;
 constexpr int kScoreRow = 80;  // bytes of a row of 32 bf16 scores in LDS, spread over the banks
 
-// 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key: eight consecutive rows read at one chunk, and four
-// rows read at a pair of chunks by the transposing loads, fall on distinct banks.
+// 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key: sixteen consecutive rows read at one chunk, and four
+// rows read by the transposing loads at a pair or an aligned group of four chunks, fall on distinct banks (a row of 128 elements
+// spans all of them, one of 64 half).
 template <int WIDTH>
 __device__ __forceinline__ int tile_key(int row) {
-  if constexpr (WIDTH >= 128) return (row & 7) << 1;
-  else return ((row >> 1) & 3) << 1;
+  if constexpr (WIDTH >= 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
 typedef __attribute__((address_space(3))) const char lds_char;
@@ -135,17 +136,13 @@ __device__ __forceinline__ u32x2 lds_read_columns(uint32_t at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
 }
 
-// Where a lane reads a tile of rows of WIDTH elements.  The XOR of a chunk number with the row's key splits into the lane's part,
-// held in a few registers, and parts that are the same for all lanes and become the reads' immediate offsets.
+// Where a lane reads a tile of rows of WIDTH elements.  Chunk 4 s + c of a row lies at the lane's address for chunk c with bits 6 and
+// up XOR-ed with s (tiles start at multiples of 1 KiB): one register a pattern.
 template <int WIDTH>
-struct TileRows {  // row i (of sixteen, more a constant further on), eight elements from 32 ks + 8 g on
-  static constexpr int N = WIDTH >= 128 ? 4 : WIDTH / 32;
-  uint32_t at[N];
-  __device__ __forceinline__ void init(int i16, int g4) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) at[k] = i16 * WIDTH * 2 + (((4 * k + g4) ^ tile_key<WIDTH>(i16)) << 4);
-  }
-  __device__ __forceinline__ u32x4 read(uint32_t tile, int row16, int ks) const { return lds_read(tile + at[ks % N] + (ks / N) * (N * 64) + row16 * 16 * WIDTH * 2); }
+struct TileRows {  // row i (of sixteen, more a constant further on), eight elements from 32 s + 8 g on
+  uint32_t at;
+  __device__ __forceinline__ void init(int i16, int g4) { at = i16 * WIDTH * 2 + ((g4 ^ tile_key<WIDTH>(i16)) << 4); }
+  __device__ __forceinline__ u32x4 read(uint32_t tile, int s) const { return lds_read((tile + at) ^ (s << 6)); }
 };
 template <int WIDTH>
 struct TileColumns {  // rows 8 g .. 8 g + 7 of the columns that the transposing reads hand out, four of them from this lane's address on
@@ -164,18 +161,17 @@ struct TileColumns {  // rows 8 g .. 8 g + 7 of the columns that the transposing
   }
 };
 template <int WIDTH>
-struct TileKeys {  // the same for columns 32 s + 8 (lane & 3) + 4 odd: chunk 4 s + (lane & 3), whose lane part is below 8 (4 for narrow rows)
-  uint32_t at[2];  // at[x]: the chunk's lane part, bit 2 flipped for odd s where the key reaches it
+struct TileKeys {  // the same rows of columns 32 s + 8 (lane & 3) + 4 odd
+  uint32_t at[2];
   __device__ __forceinline__ void init(int g4, int lane) {
-    const int row = 8 * g4 + ((lane & 15) >> 2), part = (lane & 3) ^ tile_key<WIDTH>(row);
-    at[0] = row * WIDTH * 2 + (part << 4);
-    at[1] = row * WIDTH * 2 + ((part ^ 4) << 4);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int row = 8 * g4 + ((lane & 15) >> 2) + 4 * y;
+      at[y] = row * WIDTH * 2 + (((lane & 3) ^ tile_key<WIDTH>(row)) << 4);
+    }
   }
   __device__ __forceinline__ u32x4 read(uint32_t tile, int s, int odd) const {
-    // the key of the row four further on differs in bit 3 of the chunk (wide rows) or bit 2 (narrow ones)
-    const int sx = s, sy = WIDTH >= 128 ? s ^ 2 : s ^ 1;
-    const u32x2 x = lds_read_columns(tile + (WIDTH >= 128 ? at[sx & 1] + (sx >> 1) * 128 : at[sx & 1]) + 8 * odd);
-    const u32x2 y = lds_read_columns(tile + (WIDTH >= 128 ? at[sy & 1] + (sy >> 1) * 128 : at[sy & 1]) + 8 * odd + 4 * WIDTH * 2);
+    const u32x2 x = lds_read_columns(((tile + at[0]) ^ (s << 6)) + 8 * odd), y = lds_read_columns(((tile + at[1]) ^ (s << 6)) + 8 * odd);
     return u32x4{x[0], x[1], y[0], y[1]};
   }
 };
@@ -188,13 +184,12 @@ __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(
 __device__ uint4 decay_zeros;  // 16 bytes of zeros: the source of what a tile holds beyond its rows and columns
 
 // A tile of kChunk rows of WIDTH elements on its way into LDS: rows 0 .. n-1 of `cols` elements exist, `stride` elements apart, the
-// others become zeros.  VEC: direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's vector-memory
-// counter says so; a whole tile takes its lanes' offsets from registers and its base from scalars.  Otherwise rows at any
-// address, element by element, complete at the next barrier.
-template <int WIDTH, int NT, bool VEC>
+// others become zeros.  Direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's vector-memory counter
+// says so; a whole tile takes its lanes' offsets from registers and its base from scalars.
+template <int WIDTH, int NT>
 struct TileLoad {
   static constexpr int PER_ROW = WIDTH / 8, PIECES = kChunk * PER_ROW, N = PIECES >= NT ? PIECES / NT : 1;  // fewer pieces than threads: the first waves'
-  uint32_t at[VEC ? N : 1];
+  uint32_t at[N];
   int64_t stride;
   int cols;
   // wave w's instruction k fills bytes [(w N + k) 1024, + 1024) of the tile
@@ -202,40 +197,21 @@ struct TileLoad {
   static __device__ __forceinline__ int column(int k) { return ((piece(k) % PER_ROW) ^ tile_key<WIDTH>(piece(k) / PER_ROW)) * 8; }
   __device__ __forceinline__ void init(int64_t stride_, int cols_) {
     stride = stride_; cols = cols_;
-    if constexpr (VEC) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) at[k] = ((uint32_t)(piece(k) / PER_ROW) * (uint32_t)stride + column(k)) * 2;  // 32 rows span less than 2^31 bytes
-    }
+    for (int k = 0; k < N; ++k) at[k] = ((uint32_t)(piece(k) / PER_ROW) * (uint32_t)stride + column(k)) * 2;  // 32 rows span less than 2^31 bytes
   }
   __device__ __forceinline__ void start(char* tile, const uint16_t* src, int n) const {
     if (PIECES < NT && (int)threadIdx.x >= PIECES) return;
-    if constexpr (VEC) {
-      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + (threadIdx.x >> 6) * N * 1024);
-      if (n >= kChunk && cols >= WIDTH) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tile) + (threadIdx.x >> 6) * N * 1024);
+    if (n >= kChunk && cols >= WIDTH) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) dma16(to + k * 1024, at[k], src);
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int row = piece(k) / PER_ROW, c = column(k);
-          const void* from = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
-          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + k * 1024), "v"(from) : "memory");
-        }
-      }
+      for (int k = 0; k < N; ++k) dma16(to + k * 1024, at[k], src);
     } else {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         const int row = piece(k) / PER_ROW, c = column(k);
-        uint64_t lo = 0, hi = 0;
-        if (row < n) {
-          const uint16_t* from = src + row * stride + c;
-#pragma unroll 1
-          for (int x = min(cols - c, 8) - 1; x >= 0; --x) {
-            hi = (hi << 16) | (lo >> 48);
-            lo = (lo << 16) | from[x];
-          }
-        }
-        *(u32x4*)(tile + piece(k) * 16) = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        const void* from = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + k * 1024), "v"(from) : "memory");
       }
     }
   }
@@ -261,7 +237,7 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return w;
 }
 
-template <int DK, int NW, bool OUT, bool VEC>
+template <int DK, int NW, bool OUT>
 __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
   constexpr int NT = 64 * NW, DV = 16 * NW, ND = DK / 16;
   constexpr int KB = kChunk * DK * 2, VB = kChunk * DV * 2;
@@ -282,8 +258,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
   const uint16_t* k = (const uint16_t*)p.k + (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk;
   const uint16_t* v = (const uint16_t*)p.v + (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
   const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
-  TileLoad<DK, NT, VEC> lq, lk;
-  TileLoad<DV, NT, VEC> lv;
+  TileLoad<DK, NT> lq, lk;
+  TileLoad<DV, NT> lv;
   lk.init(p.k_stride, p.Dk);
   lv.init(p.v_stride, vcols);
   const int64_t first = OUT ? 0 : (int64_t)(chunks - 1) * kChunk;
@@ -340,10 +316,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
       const int step = c * groups + gq;
       // this step's tiles have arrived, and the other buffers have been read.  Behind the tiles' loads this wave issued the two
       // stores of the step before where it holds 16 columns (`whole`): they need not be waited for.
-      if constexpr (VEC) {
-        if (whole && step > 0) wait_loads<2>();
-        else wait_loads<0>();
-      }
+      if (whole && step > 0) wait_loads<2>();
+      else wait_loads<0>();
       __syncthreads();
       const bool on = gq == groups - 1;  // the next step is another chunk's
       const int cn = c + (on ? 1 : 0);
@@ -365,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
           f32x4 acc = {};
 #pragma unroll
           for (int ks = 0; ks < DK / 32; ++ks)
-            acc = mfma_bf16(rows.read(tK + a * 16 * DK * 2, 0, ks), rows.read(tQ + b * 16 * DK * 2, 0, ks), acc);
+            acc = mfma_bf16(rows.read(tK + a * 16 * DK * 2, ks), rows.read(tQ + b * 16 * DK * 2, ks), acc);
           const int t = 16 * b + i16, s0 = 16 * a + 4 * g4;
           float f[4];
 #pragma unroll
@@ -382,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
           const u32x4 st = {pack_bf16(S[2 * s][0], S[2 * s][1]), pack_bf16(S[2 * s][2], S[2 * s][3]),
                             pack_bf16(S[2 * s + 1][0], S[2 * s + 1][1]), pack_bf16(S[2 * s + 1][2], S[2 * s + 1][3])};
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(st, rows.read(tQ, tt, s), o[tt]);
+          for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(st, rows.read(tQ + tt * 16 * DK * 2, s), o[tt]);
         }
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) o[tt] *= pw[16 * tt + i16 + 1];
@@ -471,31 +445,277 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
     }
 }
 
-template <int DK, int NW, bool VEC>
-void launch_bf16(hipStream_t stream, const DecayParams& p) {
-  const int slices = (p.Dv + 16 * NW - 1) / (16 * NW), heads = p.Hkv * slices;
-  if (p.slots > 0) {
-    hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false, VEC>), dim3(p.slots * heads), dim3(64 * NW), 0, stream, p);
-    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
+// ---- float32 and half, and bf16 rows that are not aligned: matrix instructions on float32 operands --------------------------
+// The same chunks, tiles and owners with 16 x 16 x 4 float32 instructions (a sixteenth of the bf16 rate), elements widened to
+// float32 on their way into LDS.  Nothing is rounded on the way, and any row the checks allow can be read; the tiles of the next
+// chunk wait in registers (six pieces of four elements a thread at 128 keys).  Lane (i, g), register j of tile d of the state: key
+// 16 d + 4 g + j of column i.
+constexpr int kWidePad = 4;  // floats behind a row of LDS: rows start four banks apart
+
+template <int DT>
+__device__ __forceinline__ float4 load_four(const void* src, int64_t at, bool vec) {
+  float f[4];
+  if constexpr (DT == RPA_F32) {
+    if (vec) return *(const float4*)((const float*)src + at);
+  } else if (vec) {
+    const u32x2 w = *(const u32x2*)((const uint16_t*)src + at);
+    if constexpr (DT == RPA_BF16) {
+      return make_float4(low_half(w[0]), high_half(w[0]), low_half(w[1]), high_half(w[1]));
+    } else {
+      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+      const f16x4 x = __builtin_bit_cast(f16x4, w);
+      return make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+    }
   }
-  hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true, VEC>), dim3((p.first_ids + p.slots) * heads), dim3(64 * NW), 0, stream, p);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = load_elem<DT>(src, at + e);
+  return make_float4(f[0], f[1], f[2], f[3]);
 }
 
-template <int DK>
-void launch_bf16_cols(hipStream_t stream, const DecayParams& p) {
-  if (!p.vec) launch_bf16<DK, 8, false>(stream, p);
-  else if (p.Dv <= 64) launch_bf16<DK, 4, true>(stream, p);
-  else launch_bf16<DK, 8, true>(stream, p);
+template <int DT, int WIDTH, int NT>
+struct WideTile {
+  static constexpr int PER_ROW = WIDTH / 4, N = kChunk * PER_ROW / NT, PITCH = WIDTH + kWidePad;
+  float4 r[N];
+  __device__ __forceinline__ void load(const void* src, int64_t at, int64_t stride, int n, int cols, bool vec) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int idx = threadIdx.x + k * NT, row = idx / PER_ROW, c = (idx % PER_ROW) * 4;
+      const bool in = row < n && c < cols;
+      const float4 x = load_four<DT>(src, at + (in ? row * stride + c : 0), vec);  // unconditional: all in flight at once
+      r[k] = in ? x : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  __device__ __forceinline__ void store(float* tile) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int idx = threadIdx.x + k * NT, row = idx / PER_ROW, c = (idx % PER_ROW) * 4;
+      *(float4*)(tile + row * PITCH + c) = r[k];
+    }
+  }
+};
+
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <int DT, int DK, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p) {
+  constexpr int NT = 64 * NW, DV = 16 * NW, ND = DK / 16;
+  constexpr int KP = DK + kWidePad, VP = DV + kWidePad, PP = kChunk + kWidePad;
+  __shared__ __align__(16) float sQ[OUT ? kChunk * KP : 4];
+  __shared__ __align__(16) float sK[kChunk * KP];
+  __shared__ __align__(16) float sV[kChunk * VP];
+  __shared__ __align__(16) float sP[OUT ? kChunk * PP : 4];
+  __shared__ __align__(16) float pw[kChunk + 4];
+  __shared__ __align__(16) float left[kChunk];
+
+  const int slices = (p.Dv + DV - 1) / DV, heads = p.Hkv * slices;
+  const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
+  Segment g;
+  if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, i16 = lane & 15, g4 = lane >> 4;
+  const int chunks = (g.n + kChunk - 1) / kChunk;
+  const int vcols = min(p.Dv - c0, DV), groups = OUT ? p.group : 1;
+  const int64_t q0 = (int64_t)g.t0 * p.q_stride + (int64_t)h * p.group * p.Dk, k0 = (int64_t)g.t0 * p.k_stride + (int64_t)h * p.Dk,
+                v0 = (int64_t)g.t0 * p.v_stride + (int64_t)h * p.Dv + c0;
+  WideTile<DT, DK, NT> nq, nk;
+  WideTile<DT, DV, NT> nv;
+  const int64_t first = OUT ? 0 : (int64_t)(chunks - 1) * kChunk;  // states alone: last chunk first
+  if constexpr (OUT) nq.load(p.q, q0, p.q_stride, g.n, p.Dk, p.vec);
+  nk.load(p.k, k0 + first * p.k_stride, p.k_stride, g.n, p.Dk, p.vec);
+  nv.load(p.v, v0 + first * p.v_stride, p.v_stride, g.n, vcols, p.vec);
+
+  const int col = c0 + 16 * w + i16;
+  const bool mine = col < p.Dv;
+  f32x4 S[ND];
+  const float* from = OUT ? state_ahead(p, g, h) : nullptr;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) S[d] = f32x4{};
+  if (from != nullptr) {
+    const float* at = from + (mine ? col : 0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = 16 * d + 4 * g4 + j;
+        const float x = at[min(key, p.Dk - 1) * p.Dv];
+        S[d][j] = mine && key < p.Dk ? x : 0.f;
+      }
+  }
+  const float rate = p.log_decay[h];
+  const float2 full = decay_power(rate, kChunk);
+  const float per = full.x > 0.f ? 1.f / full.x : 0.f;
+  float off = 0.f;
+  double over = 1.0;
+  if (tid <= kChunk) pw[tid] = decay_float(rate, tid);
+  if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_float(rate, kChunk - 1 - (tid - 64));
+  if constexpr (OUT) {
+    if (tid >= 128 && tid < 192) *(float4*)(sP + (tid & 15) * PP + 16 + ((tid >> 4) & 3) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+
+  for (int c = 0; c < chunks; ++c) {
+    const int n = OUT ? min(g.n - c * kChunk, kChunk) : kChunk;
+    float vv[2][4];  // tokens 16 b + 4 g + e of column i
+    for (int gq = 0; gq < groups; ++gq) {
+      __syncthreads();  // the tiles of the step before have been read
+      if constexpr (OUT) nq.store(sQ);
+      if (gq == 0) {
+        nk.store(sK);
+        nv.store(sV);
+        if (n < kChunk && tid < kChunk) left[tid] = tid < n ? pw[n - 1 - tid] : 0.f;
+      }
+      __syncthreads();
+      const bool on = gq == groups - 1;
+      const int cn = c + (on ? 1 : 0);
+      if (cn < chunks) {
+        const int64_t ahead = (int64_t)(OUT ? cn : chunks - 1 - cn) * kChunk;
+        const int rows = OUT ? g.n - cn * kChunk : kChunk;
+        if constexpr (OUT) nq.load(p.q, q0 + ahead * p.q_stride + (on ? 0 : (gq + 1) * p.Dk), p.q_stride, rows, p.Dk, p.vec);
+        if (on) {
+          nk.load(p.k, k0 + ahead * p.k_stride, p.k_stride, rows, p.Dk, p.vec);
+          nv.load(p.v, v0 + ahead * p.v_stride, p.v_stride, rows, vcols, p.vec);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vv[b][e] = sV[(16 * b + 4 * g4 + e) * VP + 16 * w + i16];
+      if constexpr (OUT) {
+        if (w < 3) {  // scores: tile (keys 16 a.., queries 16 b..) of S^T
+          const int a = w == 1 ? 1 : 0, b = w == 0 ? 0 : 1;
+          f32x4 acc = {};
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const float4 x = *(const float4*)&sK[(16 * a + i16) * KP + 16 * d + 4 * g4], y = *(const float4*)&sQ[(16 * b + i16) * KP + 16 * d + 4 * g4];
+            acc = mfma_f32(x.x, y.x, acc); acc = mfma_f32(x.y, y.y, acc); acc = mfma_f32(x.z, y.z, acc); acc = mfma_f32(x.w, y.w, acc);
+          }
+          const int t = 16 * b + i16, s0 = 16 * a + 4 * g4;
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int gap = t - s0 - e;
+            f[e] = gap >= 0 ? acc[e] * pw[max(gap, 0)] : 0.f;
+          }
+          *(float4*)&sP[t * PP + s0] = make_float4(f[0], f[1], f[2], f[3]);
+        }
+        f32x4 o[2] = {};
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const float4 y = *(const float4*)&sQ[(16 * tt + i16) * KP + 16 * d + 4 * g4];
+            o[tt] = mfma_f32(S[d][0], y.x, o[tt]); o[tt] = mfma_f32(S[d][1], y.y, o[tt]);
+            o[tt] = mfma_f32(S[d][2], y.z, o[tt]); o[tt] = mfma_f32(S[d][3], y.w, o[tt]);
+          }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) o[tt] *= pw[16 * tt + i16 + 1];
+        bool fine = true;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) fine = fine && __builtin_isfinite(vv[b][e]);
+        const bool odd = __any(!fine);  // as in the bf16 kernel: kept out of the product, NaN by hand
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int tt = b; tt < 2; ++tt) {
+            const float4 y = *(const float4*)&sP[(16 * tt + i16) * PP + 16 * b + 4 * g4];
+            const float s4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[tt] = mfma_f32(odd && !__builtin_isfinite(vv[b][e]) ? 0.f : vv[b][e], s4[e], o[tt]);
+          }
+        if (odd) {
+          int bad = 0;
+          for (; bad < n; ++bad)
+            if (!__builtin_isfinite(sV[bad * VP + 16 * w + i16])) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int first_bad = __shfl(bad, 4 * g4 + j);
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) o[tt][j] = 16 * tt + i16 >= first_bad ? __builtin_nanf("") : o[tt][j];
+          }
+        }
+        const int at = c0 + 16 * w + 4 * g4;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const int t = 16 * tt + i16;
+          if (t >= n || at >= p.Dv) continue;
+          const int64_t to = ((int64_t)(g.t0 + c * kChunk + t) * p.Hq + h * p.group + gq) * p.Dv + at;
+          const f32x4 x = o[tt] * p.scale;
+          if constexpr (DT == RPA_F32) *(f32x4*)((float*)p.out + to) = x;
+          else *(u32x2*)((uint16_t*)p.out + to) = u32x2{Half16<DT>::pack(x[0], x[1]), Half16<DT>::pack(x[2], x[3])};
+        }
+      }
+    }
+    if (OUT && c == chunks - 1 && (!g.last || g.out < 0)) break;  // nobody reads the state behind this chunk
+    float behind = 1.f;
+    if constexpr (OUT) {
+      const float l = n < kChunk ? pw[n] : full.x + (full.y - full.x * off);
+      off += ((l - full.x) - full.y) * per;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) S[d] *= l;
+    } else {
+      behind = (float)over;
+      over *= (double)full.x + (double)full.y;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float4 lf = *(const float4*)&left[16 * b + 4 * g4];
+      const float l4[4] = {lf.x, lf.y, lf.z, lf.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = vv[b][e] * (l4[e] * behind);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma_f32(sK[(16 * b + 4 * g4 + e) * KP + 16 * d + i16], x, S[d]);
+      }
+    }
+  }
+  if (OUT && (!g.last || g.out < 0)) return;
+  if (!mine) return;
+  float* at = (OUT ? p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv : scratch_state(p, g.base + g.j, h)) + col;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = 16 * d + 4 * g4 + j;
+      if (key < p.Dk) at[key * p.Dv] = S[d][j];
+    }
+}
+
+// Rows of 16-byte aligned bf16 take the bf16 kernel, everything else the float32 one; eight waves (128 columns) a workgroup, four
+// where the values have at most 64.
+template <int DT, int DK, int NW, bool DIRECT>
+void launch_tiles(hipStream_t stream, const DecayParams& p) {
+  const int slices = (p.Dv + 16 * NW - 1) / (16 * NW), heads = p.Hkv * slices;
+  const dim3 block(64 * NW), sums(p.slots * heads), outs((p.first_ids + p.slots) * heads);
+  if (p.slots > 0) {
+    if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), sums, block, 0, stream, p);
+    else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, false>), sums, block, 0, stream, p);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
+  }
+  if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true>), outs, block, 0, stream, p);
+  else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, true>), outs, block, 0, stream, p);
+}
+
+template <int DT, int DK, bool DIRECT>
+void launch_columns(hipStream_t stream, const DecayParams& p) {
+  if (p.Dv <= 64) launch_tiles<DT, DK, 4, DIRECT>(stream, p);
+  else launch_tiles<DT, DK, 8, DIRECT>(stream, p);
+}
+
+template <int DT, bool DIRECT>
+void launch_keys(hipStream_t stream, const DecayParams& p) {
+  if (p.Dk <= 64) launch_columns<DT, 64, DIRECT>(stream, p);
+  else if (p.Dk <= 128) launch_columns<DT, 128, DIRECT>(stream, p);
+  else launch_columns<DT, 256, DIRECT>(stream, p);
 }
 
 }  // namespace
 
-bool decay_chunk_supported(const DecayParams& p) { return p.dtype == RPA_BF16; }
-
 int launch_decay_chunk(hipStream_t stream, const DecayParams& p) {
-  if (p.Dk <= 64) launch_bf16_cols<64>(stream, p);
-  else if (p.Dk <= 128) launch_bf16_cols<128>(stream, p);
-  else launch_bf16_cols<256>(stream, p);
+  if (p.dtype == RPA_BF16 && p.vec) launch_keys<RPA_BF16, true>(stream, p);
+  else if (p.dtype == RPA_BF16) launch_keys<RPA_BF16, false>(stream, p);
+  else if (p.dtype == RPA_F16) launch_keys<RPA_F16, false>(stream, p);
+  else launch_keys<RPA_F32, false>(stream, p);
   return (int)hipGetLastError();
 }
 
