@@ -963,7 +963,7 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   if (Dk % 4 != 0 || Dv % 4 != 0 || Dk > 256 || Dv > 256)
     return fail(RPA_ERR_UNSUPPORTED, "%s: key size %d / value size %d (want multiples of 4, at most 256)", who, Dk, Dv);
   if (dtype != RPA_F32 && dtype != RPA_BF16 && dtype != RPA_F16) return fail(RPA_ERR_UNSUPPORTED, "%s: dtype %d (want f32, bf16 or f16)", who, dtype);
-  if (S > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: %d sequences (at most 65535)", who, S);
+  if (S > 65000) return fail(RPA_ERR_UNSUPPORTED, "%s: %d sequences (at most 65000)", who, S);
   if (!std::isfinite(scale)) return fail(RPA_ERR_INVALID_ARGUMENT, "%s: scale is not finite", who);
   if (const int rc = check_strides(who, query_stride, (int64_t)Hq * Dk, key_stride, (int64_t)Hkv * Dk, value_stride, (int64_t)Hkv * Dv)) return rc;
   if (T == 0) return RPA_OK;

@@ -10,12 +10,40 @@ namespace rpa {
 
 namespace {
 
+// A state is next wanted a whole model's worth of traffic later: past the caches, reads and writes stream faster (256 states of 64
+// heads of 128 x 128: 393 -> 374 us, 5.8 TB/s).
+__device__ __forceinline__ float4 load_once(const float* at) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  const f4 x = __builtin_nontemporal_load((const f4*)at);
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store_once(float* at, const float4& v) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  const f4 x = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(x, (f4*)at);
+}
+
+// Zeros in the output rows of tokens that belong to no sequence, shared out over `blocks` workgroups.
+template <int DT>
+__device__ __forceinline__ void clear_padded_rows(const DecayParams& p, int block, int blocks) {
+  const int n = decay_live_rows(p), lo = n > 0 ? min(max(p.qsl[0], 0), p.T) : p.T, hi = n > 0 ? min(max(p.qsl[n], lo), p.T) : p.T;
+  const int64_t row = (int64_t)p.Hq * p.Dv * ElemBytes<DT>::v / 8;  // 8 bytes at a time: rows are multiples of four elements
+  for (int r = block; r < lo + (p.T - hi); r += blocks) {
+    uint2* at = (uint2*)p.out + (int64_t)(r < lo ? r : hi + (r - lo)) * row;
+    for (int64_t k = threadIdx.x; k < row; k += blockDim.x) at[k] = make_uint2(0u, 0u);
+  }
+}
+
 template <int DT, int CG, int NR>  // CG groups of four columns, NR rows per thread
 __global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayParams p) {
   constexpr int RG = 256 / CG;
-  constexpr int MAXD = 256;
+  constexpr int MAXD = 256;  // keys at most
   __shared__ float sk[MAXD], sq[MAXD], sv[4 * CG];
   __shared__ float4 part[4][CG];
+  if ((int)blockIdx.y >= p.S) {
+    clear_padded_rows<DT>(p, (blockIdx.y - p.S) * gridDim.x + blockIdx.x, (gridDim.y - p.S) * gridDim.x);
+    return;
+  }
   const int i = blockIdx.y, slices = (p.Dv + 4 * CG - 1) / (4 * CG);
   const int h = blockIdx.x / slices, c0 = (blockIdx.x - h * slices) * 4 * CG;
   const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
@@ -29,7 +57,7 @@ __global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayParams p) {
   for (int j = 0; j < NR; ++j) {
     const int r = rg + j * RG;
     S[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (s.in >= 0 && in_cols && r < p.Dk) S[j] = *(const float4*)(p.state + (int64_t)s.in * p.Hkv * head + at + (int64_t)r * p.Dv);
+    if (s.in >= 0 && in_cols && r < p.Dk) S[j] = load_once(p.state + (int64_t)s.in * p.Hkv * head + at + (int64_t)r * p.Dv);
   }
   const float2 l = decay_power(p.log_decay[h], 1);
   for (int n = 0; n < s.q_len; ++n) {
@@ -76,23 +104,16 @@ __global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayParams p) {
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     const int r = rg + j * RG;
-    if (r < p.Dk) *(float4*)(p.state + (int64_t)s.out * p.Hkv * head + at + (int64_t)r * p.Dv) = S[j];
+    if (r < p.Dk) store_once(p.state + (int64_t)s.out * p.Hkv * head + at + (int64_t)r * p.Dv, S[j]);
   }
-}
-
-// Rows of tokens that belong to no sequence.
-__global__ __launch_bounds__(256) void decay_pad_kernel(DecayParams p, int row_bytes) {
-  const int t = blockIdx.x, n = decay_live_rows(p);
-  if (n > 0 && t >= p.qsl[0] && t < p.qsl[n]) return;
-  uint32_t* row = (uint32_t*)((char*)p.out + (int64_t)t * row_bytes);
-  for (int k = threadIdx.x; k < row_bytes / 4; k += 256) row[k] = 0u;
 }
 
 template <int DT, int CG>
 int launch_cols(hipStream_t stream, const DecayParams& p) {
   constexpr int RG = 256 / CG;
   const int slices = (p.Dv + 4 * CG - 1) / (4 * CG);
-  const dim3 grid(p.Hkv * slices, p.S), block(256);
+  const int wide = p.Hkv * slices;
+  const dim3 grid(wide, p.S + (256 + wide - 1) / wide), block(256);  // the last rows of workgroups clear padded rows
   const int need = (p.Dk + RG - 1) / RG;
   if (need <= 64 / RG) hipLaunchKernelGGL((decay_recurrent_kernel<DT, CG, 64 / RG>), grid, block, 0, stream, p);
   else if (need <= 128 / RG) hipLaunchKernelGGL((decay_recurrent_kernel<DT, CG, 128 / RG>), grid, block, 0, stream, p);
@@ -102,12 +123,18 @@ int launch_cols(hipStream_t stream, const DecayParams& p) {
 
 }  // namespace
 
+// A workgroup takes 128 columns of a state where the bounds allow four workgroups a CU or more, and 32 below that, for more of
+// them: 256 states of 64 heads of 128 x 128 374 against 398 us, 8 states of 32 heads 8.5 against 7.8 us.
+template <int DT>
+static int launch_recurrent(hipStream_t stream, const DecayParams& p) {
+  return (int64_t)p.S * p.Hkv >= 1024 ? launch_cols<DT, 32>(stream, p) : launch_cols<DT, 8>(stream, p);
+}
+
 int launch_decay_recurrent(hipStream_t stream, const DecayParams& p) {
-  hipLaunchKernelGGL(decay_pad_kernel, dim3(p.T), dim3(256), 0, stream, p, p.Hq * p.Dv * elem_bytes(p.dtype));
   switch (p.dtype) {
-    case RPA_F32: return launch_cols<RPA_F32, 8>(stream, p);
-    case RPA_BF16: return launch_cols<RPA_BF16, 8>(stream, p);
-    case RPA_F16: return launch_cols<RPA_F16, 8>(stream, p);
+    case RPA_F32: return launch_recurrent<RPA_F32>(stream, p);
+    case RPA_BF16: return launch_recurrent<RPA_BF16>(stream, p);
+    case RPA_F16: return launch_recurrent<RPA_F16>(stream, p);
     default: return (int)hipErrorInvalidValue;
   }
 }

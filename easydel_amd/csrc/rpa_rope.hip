@@ -248,13 +248,17 @@ __device__ __forceinline__ int find_run_wave(const int32_t* qsl, int n, int page
 
 // A run is the new tokens one sequence writes to one page.  Runs are numbered without a plan: a sequence of n tokens from
 // qsl[i] on touches at most (n - 1) / page_size + 2 pages, and floor(qsl[i] / page_size) + 2 i leaves room for as many
-// ahead of the next sequence's first number.  One wave codes one run of one combined head by the rule of the quantising
-// scatter: amax over the (turned) values, the new scale, old codes again if it grew, new codes.  The values are turned twice
-// rather than held: the second reading comes from the caches.
+// ahead of the next sequence's first number.  One workgroup codes one run of one combined head by the rule of the quantising
+// scatter: amax over the (turned) values, the new scale, old codes again if it grew, new codes.  Its threads hold the turned
+// values between the maximum and the codes (64 tokens of 128 elements: four pieces of eight a thread); of longer runs the
+// pieces behind those are read and turned again, from the caches.  (A wave a run, with everything turned twice: 64 decode rows
+// and 2048 prompt tokens of 8 heads into fp8 pages took 37 us, which its chain of loads bounded.)
+constexpr int kHold = 4;
+
 template <int SRC, int KVT, int VEC>
-__device__ __forceinline__ void append_run(const RopeParams& p, int n_live, int run, int c) {
+__device__ __forceinline__ void append_run(const RopeParams& p, int n_live, int run, int c, float* most) {
   constexpr int E = ElemBytes<SRC>::v;
-  const int lane = threadIdx.x & 63;
+  const int tid = threadIdx.x;
   const int i = find_run_wave(p.qsl, n_live, p.page_size, run);
   const int q0 = p.qsl[i], q_len = p.qsl[i + 1] - q0;
   const int ctx = p.context_lens[i];
@@ -271,65 +275,95 @@ __device__ __forceinline__ void append_run(const RopeParams& p, int n_live, int 
   const int n = min(min(ctx, (int)begin + p.page_size) - pos, p.T - t0);
   if (n <= 0) return;
   const bool key = !(c & 1);
-  const int h = c >> 1, half = p.rope >> 1, per = p.D / (2 * VEC);
+  const int h = c >> 1, half = p.rope >> 1, per = p.D / (2 * VEC), pieces = n * per;
   const int64_t stride = key ? p.k_stride : p.v_stride;
   const char* src = (const char*)(key ? p.k : p.v) + ((int64_t)t0 * stride + (int64_t)h * p.D) * E;
   unsigned char* dst = (unsigned char*)p.k_pages + (int64_t)page * p.page_stride + (int64_t)c * p.Dp;
   const int64_t dst_row = p.token_stride;
-  float f[2 * VEC];
-  int d0, d1;
+  const int64_t si = (int64_t)page * p.C + c;
+  const float old_scale = first == 0 ? 0.f : p.scales[si];
+  float held[kHold][2 * VEC];
 
   float amax = 0.f;
-  for (int k = lane; k < n * per; k += 64) {
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int k = tid + u * 256;
+    if (k < pieces) {
+      const int r = k / per, piece = k - r * per;
+      int d0, d1;
+      load_piece<SRC, VEC>(src + r * stride * E, angle_row(p, t0 + r, pos + r), half, p.neox, piece, key, held[u], d0, d1);
+#pragma unroll
+      for (int e = 0; e < 2 * VEC; ++e) amax = fmaxf(amax, fabsf(held[u][e]));
+    }
+  }
+  for (int k = tid + kHold * 256; k < pieces; k += 256) {
     const int r = k / per, piece = k - r * per;
+    float f[2 * VEC];
+    int d0, d1;
     load_piece<SRC, VEC>(src + r * stride * E, angle_row(p, t0 + r, pos + r), half, p.neox, piece, key, f, d0, d1);
 #pragma unroll
     for (int e = 0; e < 2 * VEC; ++e) amax = fmaxf(amax, fabsf(f[e]));
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  if ((tid & 63) == 0) most[tid >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
   constexpr float unit = KVT == RPA_FP8_E4M3 ? 1.f / 448.f : 1.f / 127.f;
-  const int64_t si = (int64_t)page * p.C + c;
-  const float old_scale = first == 0 ? 0.f : p.scales[si];
   float new_scale = fmaxf(old_scale, amax * unit);
   if (new_scale == 0.f) new_scale = 1.f;
 
   if (new_scale > old_scale && first > 0) {
     const int words = p.D >> 2;  // head rows are multiples of four codes
-    for (int k = lane; k < first * words; k += 64) {
+    for (int k = tid; k < first * words; k += 256) {
       const int r = k / words, d = (k - r * words) * 4;
       uint32_t* at = (uint32_t*)(dst + r * dst_row + d);
-      const uint32_t held = *at;
+      const uint32_t was = *at;
       uint32_t w = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w |= quant1<KVT>((decode1<KVT>((held >> (8 * e)) & 0xff) * old_scale) / new_scale) << (8 * e);
+      for (int e = 0; e < 4; ++e) w |= quant1<KVT>((decode1<KVT>((was >> (8 * e)) & 0xff) * old_scale) / new_scale) << (8 * e);
       *at = w;
     }
   }
-  for (int k = lane; k < n * per; k += 64) {
+  const bool split_rows = key && p.neox;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int k = tid + u * 256;
+    if (k < pieces) {
+      const int r = k / per, piece = k - r * per;
+      const bool split = split_rows && piece * VEC < half;
+      const int d0 = split ? piece * VEC : piece * 2 * VEC, d1 = split ? d0 + half : d0 + VEC;
+      unsigned char* row = dst + (first + r) * dst_row;
+      store_codes<KVT, VEC>(row + d0, held[u], new_scale);
+      store_codes<KVT, VEC>(row + d1, held[u] + VEC, new_scale);
+    }
+  }
+  for (int k = tid + kHold * 256; k < pieces; k += 256) {
     const int r = k / per, piece = k - r * per;
+    float f[2 * VEC];
+    int d0, d1;
     load_piece<SRC, VEC>(src + r * stride * E, angle_row(p, t0 + r, pos + r), half, p.neox, piece, key, f, d0, d1);
     unsigned char* row = dst + (first + r) * dst_row;
     store_codes<KVT, VEC>(row + d0, f, new_scale);
     store_codes<KVT, VEC>(row + d1, f + VEC, new_scale);
   }
   const int pad = (p.Dp - p.D) >> 2;
-  for (int k = lane; k < n * pad; k += 64) {
+  for (int k = tid; k < n * pad; k += 256) {
     const int r = k / pad, d = (k - r * pad) * 4;
     *(uint32_t*)(dst + (first + r) * dst_row + p.D + d) = 0u;
   }
-  if (lane == 0) p.scales[si] = new_scale;
+  if (tid == 0) p.scales[si] = new_scale;  // every wave has read the old one: it lies ahead of the barrier
 }
 
 template <int SRC, int KVT, int VEC>
 __global__ __launch_bounds__(256) void rope_append_quant_kernel(RopeParams p, int run_blocks) {
+  __shared__ float most[4];
   const int n_live = rope_live(p);
   if ((int)blockIdx.x < run_blocks) {
     if (n_live <= 0) return;
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int run = unit / (2 * p.Hkv), c = unit - run * 2 * p.Hkv;
+    const int run = blockIdx.x / (2 * p.Hkv), c = blockIdx.x - run * 2 * p.Hkv;
     if (run < p.qsl[0] / p.page_size) return;  // ahead of the first sequence's numbers
-    append_run<SRC, KVT, VEC>(p, n_live, run, c);
+    append_run<SRC, KVT, VEC>(p, n_live, run, c, most);
     return;
   }
   const int t = blockIdx.x - run_blocks;
@@ -440,9 +474,8 @@ int launch_plain(hipStream_t stream, const RopeParams& p) {
 
 template <int SRC, int KVT>
 int launch_quant(hipStream_t stream, const RopeParams& p) {
-  const int64_t units = ((int64_t)p.T / p.page_size + 2 * (int64_t)p.S) * 2 * p.Hkv;  // (run, combined head) pairs
-  const int64_t run_blocks = (units + 3) / 4;
-  if (units > 0x7ffffff0 || run_blocks + p.T > 0x7fffffff) return (int)hipErrorInvalidValue;
+  const int64_t run_blocks = ((int64_t)p.T / p.page_size + 2 * (int64_t)p.S) * 2 * p.Hkv;  // (run, combined head) pairs
+  if (run_blocks + p.T > 0x7fffffff) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)(run_blocks + p.T)), block(256);
   if (group_of<false>(p, 4) == 4) hipLaunchKernelGGL((rope_append_quant_kernel<SRC, KVT, 4>), grid, block, 0, stream, p, (int)run_blocks);
   else hipLaunchKernelGGL((rope_append_quant_kernel<SRC, KVT, 1>), grid, block, 0, stream, p, (int)run_blocks);

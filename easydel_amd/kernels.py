@@ -431,6 +431,13 @@ def mla_ragged_paged_attention(queries_nope, queries_pe, keys_values, keys_pe, k
 def _rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device) -> tuple[int, int]:
     """(pointer, elements between token rows) of a ``[T, heads, dim]`` or ``[T, dim]`` operand whose token rows are
     contiguous and may lie apart, as views of one projection's output do."""
+    # what a good call looks like first, in few steps: a decode step's launch waits for them
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.shape == shape:
+        if t.is_contiguous():
+            return t.data_ptr(), math.prod(shape[1:])
+        st = t.stride()
+        if len(st) == 3 and st[2] == 1 and st[1] == shape[2] and shape[0] > 1:
+            return t.data_ptr(), st[0]
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor holding device memory, got {type(t).__name__}")
     if tuple(t.shape) != tuple(shape):
@@ -449,7 +456,23 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device) 
     return t.data_ptr(), row if t.shape[0] <= 1 else t.stride(0)
 
 
+def _launch(device, fn, *args) -> None:
+    """``fn(stream, *args)`` on ``device``, its current stream, with HIP's current device set to it (the library queries and
+    launches on that)."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        code = fn(stream, *args)
+    else:
+        with torch.cuda.device(device):
+            code = fn(stream, *args)
+    if code != 0:
+        _lib.check(code)
+
+
 def _on(t: torch.Tensor, name: str, dtype: torch.dtype, device) -> int:
+    if t.dtype is dtype and t.is_contiguous() and t.get_device() == device.index:  # a good call, in few steps
+        return t.data_ptr()
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     ptr = _dev(t, name)
@@ -466,7 +489,7 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 def _turned_out(query, query_out, others, name: str):
     """The tensor the turned queries go to: a new one, the queries themselves, or one that overlaps no operand."""
     if query_out is None:
-        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        return torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
     if query_out.shape != query.shape or query_out.dtype != query.dtype or query_out.device != query.device:
         raise ValueError(f"{name} must be {list(query.shape)} {query.dtype} on {query.device}, got {list(query_out.shape)} "
                          f"{query_out.dtype} on {query_out.device}")
@@ -547,10 +570,8 @@ def rope_page_scatter_ragged(query, key, value, kv_pages, cos_sin, context_lens,
     pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
     scales = None if kv_scales is None else _on(kv_scales, "kv_scales", torch.float32, dev)
     if T > 0:
-        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
-            _lib.check(lib.rpa_rope_page_scatter_ragged(
-                _stream(query), q, k, v, out.data_ptr(), pages, scales, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, Dp, C,
-                rope, rows, int(bool(is_neox_style)), qs, ks, vs, dtype_tag(query.dtype), kd))
+        _launch(dev, lib.rpa_rope_page_scatter_ragged, q, k, v, out.data_ptr(), pages, scales, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, Dp, C,
+                rope, rows, 1 if is_neox_style else 0, qs, ks, vs, _DTYPE_TAG[query.dtype], kd)
     return (out, kv_pages) if kv_scales is None else (out, kv_pages, kv_scales)
 
 
@@ -572,10 +593,8 @@ def rope_unified_page_scatter(query, key, value, key_cache, value_cache, cos_sin
     out = _turned_out(query, query_out, (key, value), "query_out")
     kc, vc = _on(key_cache, "key_cache", key_cache.dtype, dev), _on(value_cache, "value_cache", key_cache.dtype, dev)
     if T > 0:
-        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
-            _lib.check(lib.rpa_rope_unified_page_scatter(
-                _stream(query), q, k, v, out.data_ptr(), kc, vc, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, rope, rows,
-                int(bool(is_neox_style)), qs, ks, vs, dtype_tag(query.dtype), kd))
+        _launch(dev, lib.rpa_rope_unified_page_scatter, q, k, v, out.data_ptr(), kc, vc, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, rope, rows,
+                1 if is_neox_style else 0, qs, ks, vs, _DTYPE_TAG[query.dtype], kd)
     return out, key_cache, value_cache
 
 
@@ -606,10 +625,8 @@ def rope_mla_page_scatter(queries_pe, keys_values, keys_pe, kv_pages, cos_sin, c
     out = _turned_out(queries_pe, query_out, (keys_pe, keys_values), "query_out")
     pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
     if T > 0:
-        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
-            _lib.check(lib.rpa_rope_mla_page_scatter(
-                _stream(queries_pe), q, latent, k, out.data_ptr(), pages, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, lkv, rope, row, rows,
-                int(bool(is_neox_style)), qs, ks, dtype_tag(dt), kd))
+        _launch(dev, lib.rpa_rope_mla_page_scatter, q, latent, k, out.data_ptr(), pages, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, lkv, rope, row, rows,
+                1 if is_neox_style else 0, qs, ks, _DTYPE_TAG[dt], kd)
     return out, kv_pages
 
 
@@ -641,17 +658,18 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
         raise ValueError(f"log_decay must be [{Hkv}], got {list(log_decay.shape)}")
     S = state_indices.shape[0]
     for name, t, n in (("query_start_loc", query_start_loc, S + 1), ("context_lens", context_lens, S), ("state_out_indices", state_out_indices, S)):
-        if t is not None and tuple(t.shape) != (n,):
+        if t is not None and t.shape != (n,):
             raise ValueError(f"{name} must be [{n}], got {list(t.shape)}")
     if S == 0 or num_seqs.numel() < 1:
         raise ValueError("no sequence rows")
     i32 = torch.int32
-    ptrs = [None if t is None else _on(t, name, kind, dev) for name, t, kind in (
-        ("log_decay", log_decay, torch.float32), ("state", state, torch.float32), ("state_indices", state_indices, i32),
-        ("state_out_indices", state_out_indices, i32), ("context_lens", context_lens, i32), ("query_start_loc", query_start_loc, i32),
-        ("num_seqs", num_seqs, i32))]
+    ptrs = (_on(log_decay, "log_decay", torch.float32, dev), _on(state, "state", torch.float32, dev),
+            _on(state_indices, "state_indices", i32, dev),
+            None if state_out_indices is None else _on(state_out_indices, "state_out_indices", i32, dev),
+            None if context_lens is None else _on(context_lens, "context_lens", i32, dev),
+            _on(query_start_loc, "query_start_loc", i32, dev), _on(num_seqs, "num_seqs", i32, dev))
     if out is None:
-        out = torch.empty((T, Hq, Dv), dtype=dt, device=dev)
+        out = query.new_empty((T, Hq, Dv))
     elif tuple(out.shape) != (T, Hq, Dv):
         raise ValueError(f"out must be [{T}, {Hq}, {Dv}], got {list(out.shape)}")
     else:
@@ -662,12 +680,11 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
                 raise ValueError(f"out overlaps {name}")
     o = _on(out, "out", dt, dev)
     if T > 0:
-        scale = float(Dk) ** -0.5 if scale is None else float(scale)
-        with torch.cuda.device(dev):  # the library queries and launches on HIP's current device
-            # scratch of its own for every call: the caching allocator orders its reuse by stream, and a captured graph keeps its own
-            need = int(lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, dtype_tag(dt)))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _lib.check(lib.rpa_decay_linear_attention(
-                _stream(query), q, k, v, *ptrs, o, None if ws is None else ws.data_ptr(), need, T, S, state.shape[0], Hq, Hkv, Dk, Dv,
-                qs, ks, vs, dtype_tag(dt), scale))
+        tag = _DTYPE_TAG[dt]
+        # scratch of its own for every call: the caching allocator orders its reuse by stream, and a captured graph keeps its own
+        with torch.cuda.device(dev):  # the size goes by the current device's compute units
+            need = lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, tag) if T > 1 else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _launch(dev, lib.rpa_decay_linear_attention, q, k, v, *ptrs, o, None if ws is None else ws.data_ptr(), need, T, S, state.shape[0],
+                Hq, Hkv, Dk, Dv, qs, ks, vs, tag, float(Dk) ** -0.5 if scale is None else float(scale))
     return out, state

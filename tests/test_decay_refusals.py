@@ -21,7 +21,7 @@ def _call(lib, **over):
     (dict(Dv=260, vs=520), "at most 256", -2), (dict(dt=2), "dtype", -2), (dict(dt=5), "dtype", -2), (dict(scale=float("nan")), "not finite", -1),
     (dict(scale=float("inf")), "not finite", -1), (dict(qs=511), "overlap", -1), (dict(ks=0), "overlap", -1), (dict(vs=127), "overlap", -1),
     (dict(q=None), "null", -1), (dict(g=None), "null", -1), (dict(state=None), "null", -1), (dict(si=None), "null", -1), (dict(ns=None), "null", -1),
-    (dict(out=A + 8), "16 bytes", -1), (dict(state=A + 4), "16 bytes", -1), (dict(k=A + 1), "aligned", -1), (dict(S=70000), "65535", -2)])
+    (dict(out=A + 8), "16 bytes", -1), (dict(state=A + 4), "16 bytes", -1), (dict(k=A + 1), "aligned", -1), (dict(S=70000), "65000", -2)])
 def test_the_c_entry_refuses(over, text, code):
     lib = _lib.load()
     assert _call(lib, **over) == code
