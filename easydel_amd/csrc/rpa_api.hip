@@ -939,7 +939,9 @@ static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayPara
   const int by_token = T / (rpa::kDecayRows + 1) + 1;
   p.first_by_seq = S <= by_token;
   p.first_ids = std::min(S, by_token);
-  *scratch = (size_t)2 * p.slots * Hkv * Dk * Dv * 4;
+  p.key_tiles = Dk <= 64 ? 4 : Dk <= 128 ? 8 : 16;
+  p.scratch_vecs = p.key_tiles * 64 * (Dv <= 64 ? 4 : 8 * slices);
+  *scratch = (size_t)2 * p.slots * Hkv * p.scratch_vecs * 16;
 }
 
 size_t rpa_decay_attention_workspace_bytes(int T, int S, int Hq, int Hkv, int Dk, int Dv, int dtype) {
@@ -991,10 +993,11 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
     size_t scratch;
     decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);
     p.rows = rpa::kDecayRows;
-    p.scratch = (float*)workspace;
+    p.scratch = workspace;
     const int64_t unit = 16 / e;
     p.vec = ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)value)) & 15) == 0 && query_stride % unit == 0 && key_stride % unit == 0 &&
             value_stride % unit == 0 && Dk % unit == 0 && Dv % unit == 0;
+    p.direct = dtype == RPA_BF16 && p.vec;
     const int64_t blocks = ((int64_t)p.first_ids + p.slots) * Hkv * 4;
     if (blocks > INT32_MAX || p.slots > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: T=%d tokens of %d heads are too many workgroups", who, T, Hkv);
     if (const int err = rpa::launch_decay_chunk(s, p)) return hip_fail(err, "rpa_decay_linear_attention chunk launch");

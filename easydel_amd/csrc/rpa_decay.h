@@ -27,7 +27,10 @@ struct DecayParams {
   int slots;         // scratch slots: floor(T / seg_len) + 1, 0 where no sequence can have two segments
   int first_ids;     // numbers that first segments may have ...
   int first_by_seq;  // ... which are their sequences' (1) or floor(qsl[i] / (kDecayRows + 1)) (0)
-  float* scratch;    // [2 * slots][Hkv][Dk][Dv]
+  int direct;        // the bf16 kernel serves the call (the float32 one otherwise): the order of a scratch state's keys
+  int key_tiles;     // tiles of 16 keys the kernels compute with (4, 8 or 16)
+  int scratch_vecs;  // 16-byte vectors of a scratch state: columns and keys padded to what the kernels compute with
+  void* scratch;     // [2 * slots][Hkv][scratch_vecs]
 };
 
 constexpr int kDecayRows = 16;

@@ -71,34 +71,91 @@ __device__ __forceinline__ bool find_segment(const DecayParams& p, int id, Segme
   return true;
 }
 
-__device__ __forceinline__ float* scratch_state(const DecayParams& p, int slot, int h) {
-  return p.scratch + ((int64_t)slot * p.Hkv + h) * p.Dk * p.Dv;
+// A scratch state lies as the lanes of the chunk kernels hold it, 16 bytes a lane and tile of 16 keys: [16-column group][tile][lane].
+__device__ __forceinline__ f32x4* scratch_state(const DecayParams& p, int slot, int h) {
+  return (f32x4*)p.scratch + ((int64_t)slot * p.Hkv + h) * p.scratch_vecs;
 }
 
-// Where a segment's state comes from (null: zeros).  A sequence of several segments may write the slot it started from while
-// its first segment has yet to run, so the scan keeps the state it starts from, in a second set of scratch slots.
-__device__ __forceinline__ const float* state_ahead(const DecayParams& p, const Segment& g, int h) {
-  if (g.j > 0) return scratch_state(p, g.base + g.j - 1, h);
-  if (!g.last) return scratch_state(p, p.slots + g.base, h);
-  return g.in < 0 ? nullptr : p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv;
-}
+// The first of the four keys that a lane group holds of tile d: in the order in which the bf16 kernel reads the queries, or as they
+// come (the float32 kernel).
+__device__ __forceinline__ int first_key(int direct, int d, int g4) { return direct ? 32 * (d >> 1) + 8 * g4 + 4 * (d & 1) : 16 * d + 4 * g4; }
 
-// Scratch slots hold what each segment adds to a zero state; afterwards slot base + j holds the state behind segment j.
+// Scratch slots hold what each segment adds to a zero state; afterwards slot base + j holds the state behind segment j.  A sequence
+// of several segments may write the slot of the pool it started from while its first segment has yet to run, so the state it
+// starts from is kept too, in a second set of scratch slots.
 __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
   Segment g;
   if (!find_by_slot<false>(p, blockIdx.z, g) || g.j != 0) return;
-  const int h = blockIdx.y, e = (blockIdx.x * 256 + threadIdx.x) * 4;
-  if (e >= p.Dk * p.Dv) return;
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (g.in >= 0) r = *(const float4*)(p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + e);
-  *(float4*)(scratch_state(p, p.slots + g.base, h) + e) = r;
+  const int h = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= p.scratch_vecs) return;
+  const int lane = e & 63, d = (e >> 6) % p.key_tiles, col = 16 * ((e >> 6) / p.key_tiles) + (lane & 15);
+  const int key = first_key(p.direct, d, lane >> 4);
+  f32x4 r = {};
+  if (g.in >= 0 && col < p.Dv) {
+    const float* from = p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = key + j < p.Dk ? from[(key + j) * p.Dv] : 0.f;
+  }
+  scratch_state(p, p.slots + g.base, h)[e] = r;
   const float2 l = decay_power(p.log_decay[h], p.seg_len);
-  for (int slot = g.base; slot < g.base + g.segments - 1; ++slot) {
-    float4* at = (float4*)(scratch_state(p, slot, h) + e);
-    const float4 a = *at;
-    r.x = fmaf(r.x, l.y, fmaf(r.x, l.x, a.x)); r.y = fmaf(r.y, l.y, fmaf(r.y, l.x, a.y));
-    r.z = fmaf(r.z, l.y, fmaf(r.z, l.x, a.z)); r.w = fmaf(r.w, l.y, fmaf(r.w, l.x, a.w));
-    *at = r;
+  const int end = g.base + g.segments - 1;
+  constexpr int AHEAD = 4;  // the chain is in the sums alone: the reads of several slots are in flight at once
+  for (int slot = g.base; slot < end; slot += AHEAD) {
+    f32x4 a[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) a[u] = scratch_state(p, min(slot + u, end - 1), h)[e];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (slot + u >= end) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = fmaf(r[j], l.y, fmaf(r[j], l.x, a[u][j]));
+      scratch_state(p, slot + u, h)[e] = r;
+    }
+  }
+}
+
+// The state that a segment starts from, as the lanes of one column group hold it.
+template <int ND, bool DIRECT>
+__device__ __forceinline__ void load_state(const DecayParams& p, const Segment& g, int h, int group, int lane, f32x4 (&S)[ND]) {
+  if (g.j > 0 || !g.last) {
+    const f32x4* at = scratch_state(p, g.j > 0 ? g.base + g.j - 1 : p.slots + g.base, h) + (int64_t)group * ND * 64 + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) S[d] = at[d * 64];
+    return;
+  }
+#pragma unroll
+  for (int d = 0; d < ND; ++d) S[d] = f32x4{};
+  if (g.in < 0) return;
+  const int col = 16 * group + (lane & 15);
+  const float* at = p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + min(col, p.Dv - 1);
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = first_key(DIRECT, d, lane >> 4) + j;
+      const float f = at[min(key, p.Dk - 1) * p.Dv];  // unconditional loads, all in flight at once
+      S[d][j] = col < p.Dv && key < p.Dk ? f : 0.f;
+    }
+}
+
+// The state behind a segment: into the pool (OUT, where it is a sequence's last), or what the segment added into its scratch slot.
+template <int ND, bool DIRECT, bool OUT>
+__device__ __forceinline__ void store_state(const DecayParams& p, const Segment& g, int h, int group, int lane, const f32x4 (&S)[ND]) {
+  if constexpr (!OUT) {
+    f32x4* at = scratch_state(p, g.base + g.j, h) + (int64_t)group * ND * 64 + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) at[d * 64] = S[d];
+  } else {
+    const int col = 16 * group + (lane & 15);
+    if (col >= p.Dv) return;
+    float* at = p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv + col;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = first_key(DIRECT, d, lane >> 4) + j;
+        if (key < p.Dk) at[key * p.Dv] = S[d][j];
+      }
   }
 }
 
@@ -183,6 +240,13 @@ __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(
 
 __device__ uint4 decay_zeros;  // 16 bytes of zeros: the source of what a tile holds beyond its rows and columns
 
+// A value that the compiler cannot know to be the same in every turn of a loop: what rare paths derive from it is worked out there and
+// not held in registers (or spilled, behind loads that would then be waited for) by all turns.
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // A tile of kChunk rows of WIDTH elements on its way into LDS: rows 0 .. n-1 of `cols` elements exist, `stride` elements apart, the
 // others become zeros.  Direct loads of 16 bytes a lane, 1 KiB an instruction, complete when this wave's vector-memory counter
 // says so; a whole tile takes its lanes' offsets from registers and its base from scalars.
@@ -193,12 +257,12 @@ struct TileLoad {
   int64_t stride;
   int cols;
   // wave w's instruction k fills bytes [(w N + k) 1024, + 1024) of the tile
-  static __device__ __forceinline__ int piece(int k) { return ((threadIdx.x >> 6) * N + k) * 64 + (threadIdx.x & 63); }
-  static __device__ __forceinline__ int column(int k) { return ((piece(k) % PER_ROW) ^ tile_key<WIDTH>(piece(k) / PER_ROW)) * 8; }
+  static __device__ __forceinline__ int row_of(int thread, int k) { return (((thread >> 6) * N + k) * 64 + (thread & 63)) / PER_ROW; }
+  static __device__ __forceinline__ int column_of(int thread, int k) { return (((thread & 63) % PER_ROW) ^ tile_key<WIDTH>(row_of(thread, k))) * 8; }
   __device__ __forceinline__ void init(int64_t stride_, int cols_) {
     stride = stride_; cols = cols_;
 #pragma unroll
-    for (int k = 0; k < N; ++k) at[k] = ((uint32_t)(piece(k) / PER_ROW) * (uint32_t)stride + column(k)) * 2;  // 32 rows span less than 2^31 bytes
+    for (int k = 0; k < N; ++k) at[k] = ((uint32_t)row_of(threadIdx.x, k) * (uint32_t)stride + column_of(threadIdx.x, k)) * 2;  // 32 rows span less than 2^31 bytes
   }
   __device__ __forceinline__ void start(char* tile, const uint16_t* src, int n) const {
     if (PIECES < NT && (int)threadIdx.x >= PIECES) return;
@@ -207,9 +271,10 @@ struct TileLoad {
 #pragma unroll
       for (int k = 0; k < N; ++k) dma16(to + k * 1024, at[k], src);
     } else {
+      const int thread = opaque(threadIdx.x);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const int row = piece(k) / PER_ROW, c = column(k);
+        const int row = row_of(thread, k), c = column_of(thread, k);
         const void* from = row < n && c < cols ? (const void*)(src + row * stride + c) : (const void*)&decay_zeros;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + k * 1024), "v"(from) : "memory");
       }
@@ -238,7 +303,7 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 }
 
 template <int DK, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_chunk_bf16_kernel(DecayParams p) {
+__global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_kernel(DecayParams p) {
   constexpr int NT = 64 * NW, DV = 16 * NW, ND = DK / 16;
   constexpr int KB = kChunk * DK * 2, VB = kChunk * DV * 2;
   __shared__ __align__(1024) char sK[2][KB];
@@ -270,23 +335,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
     lq.start(sQ[0], q, g.n);
   }
 
-  const int col = c0 + 16 * w + i16;
-  const bool mine = col < p.Dv;
   f32x4 S[ND];
-  const float* from = OUT ? state_ahead(p, g, h) : nullptr;
 #pragma unroll
   for (int d = 0; d < ND; ++d) S[d] = f32x4{};
-  if (from != nullptr) {
-    const float* at = from + (mine ? col : 0);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = 32 * (d >> 1) + 8 * g4 + 4 * (d & 1) + j;
-        const float x = at[min(key, p.Dk - 1) * p.Dv];  // unconditional loads, all in flight at once
-        S[d][j] = mine && key < p.Dk ? x : 0.f;
-      }
-  }
+  if constexpr (OUT) load_state<ND, true>(p, g, h, c0 / 16 + w, lane, S);
   // The state is multiplied by l^C = full.x + full.y once a chunk: each factor is rounded so that the product of all of them so
   // far stays within a rounding of the true power (`off`: how far it is, relatively), however long the segment.
   const float rate = p.log_decay[h];
@@ -340,7 +392,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
 #pragma unroll
           for (int ks = 0; ks < DK / 32; ++ks)
             acc = mfma_bf16(rows.read(tK + a * 16 * DK * 2, ks), rows.read(tQ + b * 16 * DK * 2, ks), acc);
-          const int t = 16 * b + i16, s0 = 16 * a + 4 * g4;
+          const int own = opaque(lane), t = 16 * b + (own & 15), s0 = 16 * a + 4 * (own >> 4);
           float f[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -375,7 +427,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) o[tt] = mfma_bf16(vo, lds_read(aP + (16 * tt + i16) * kScoreRow + g4 * 16), o[tt]);
         if (odd) {
-          const int at = 16 * w + i16;
+          const int at = 16 * w + (opaque(lane) & 15);
           int bad = 0;
           for (; bad < n; ++bad) {
             const uint16_t bits = *(const uint16_t*)(sV[c & 1] + bad * DV * 2 + (((at >> 3) ^ tile_key<DV>(bad)) << 4) + ((at & 7) << 1));
@@ -431,18 +483,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 16 / NW * 2 : 1) void decay_ch
     }
   }
   if (OUT && (!g.last || g.out < 0)) return;
-  float* to = OUT ? p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv : scratch_state(p, g.base + g.j, h);
-  int back = 8 * g4;
-  asm volatile("" : "+v"(back));  // the addresses and masks are not those of the beginning, kept through the loop
-  if (!mine) return;
-  float* at = to + back * p.Dv + col;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = 32 * (d >> 1) + 4 * (d & 1) + j;
-      if (key + back < p.Dk) at[key * p.Dv] = S[d][j];
-    }
+  store_state<ND, true, OUT>(p, g, h, c0 / 16 + w, opaque(lane), S);  // (addresses of its own, not those of the beginning kept through the loop)
 }
 
 // ---- float32 and half, and bf16 rows that are not aligned: matrix instructions on float32 operands --------------------------
@@ -523,23 +564,10 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
   nk.load(p.k, k0 + first * p.k_stride, p.k_stride, g.n, p.Dk, p.vec);
   nv.load(p.v, v0 + first * p.v_stride, p.v_stride, g.n, vcols, p.vec);
 
-  const int col = c0 + 16 * w + i16;
-  const bool mine = col < p.Dv;
   f32x4 S[ND];
-  const float* from = OUT ? state_ahead(p, g, h) : nullptr;
 #pragma unroll
   for (int d = 0; d < ND; ++d) S[d] = f32x4{};
-  if (from != nullptr) {
-    const float* at = from + (mine ? col : 0);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = 16 * d + 4 * g4 + j;
-        const float x = at[min(key, p.Dk - 1) * p.Dv];
-        S[d][j] = mine && key < p.Dk ? x : 0.f;
-      }
-  }
+  if constexpr (OUT) load_state<ND, false>(p, g, h, c0 / 16 + w, lane, S);
   const float rate = p.log_decay[h];
   const float2 full = decay_power(rate, kChunk);
   const float per = full.x > 0.f ? 1.f / full.x : 0.f;
@@ -670,15 +698,7 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
     }
   }
   if (OUT && (!g.last || g.out < 0)) return;
-  if (!mine) return;
-  float* at = (OUT ? p.state + ((int64_t)g.out * p.Hkv + h) * p.Dk * p.Dv : scratch_state(p, g.base + g.j, h)) + col;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = 16 * d + 4 * g4 + j;
-      if (key < p.Dk) at[key * p.Dv] = S[d][j];
-    }
+  store_state<ND, false, OUT>(p, g, h, c0 / 16 + w, opaque(lane), S);
 }
 
 // Rows of 16-byte aligned bf16 take the bf16 kernel, everything else the float32 one; eight waves (128 columns) a workgroup, four
@@ -690,7 +710,7 @@ void launch_tiles(hipStream_t stream, const DecayParams& p) {
   if (p.slots > 0) {
     if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), sums, block, 0, stream, p);
     else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, false>), sums, block, 0, stream, p);
-    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.Dk * p.Dv / 4 + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.scratch_vecs + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
   }
   if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true>), outs, block, 0, stream, p);
   else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, true>), outs, block, 0, stream, p);
