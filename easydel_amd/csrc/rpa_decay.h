@@ -24,7 +24,8 @@ struct DecayParams {
   // chunked form
   int vec;           // q, k and v rows allow 16-byte loads
   int seg_len;       // tokens of a segment
-  int slots;         // scratch slots: floor(T / seg_len) + 1, 0 where no sequence can have two segments
+  int whole_len;     // sequences of up to this many tokens (>= seg_len) are one segment
+  int slots;         // scratch slots: floor(T / seg_len) + 1, 0 where no sequence can be cut
   int first_ids;     // numbers that first segments may have ...
   int first_by_seq;  // ... which are their sequences' (1) or floor(qsl[i] / (kDecayRows + 1)) (0)
   int direct;        // the bf16 kernel serves the call (the float32 one otherwise): the order of a scratch state's keys

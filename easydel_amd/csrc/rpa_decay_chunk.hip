@@ -26,6 +26,11 @@ struct Segment {
   bool last;
 };
 
+// Sequences of up to whole_len tokens are not cut.
+__device__ __forceinline__ int segments_of(const DecayParams& p, int q_len) {
+  return q_len <= p.whole_len ? 1 : (q_len + p.seg_len - 1) / p.seg_len;
+}
+
 // The segment that scratch slot `slot` lies behind (AHEAD: the one that starts from it).
 template <bool AHEAD>
 __device__ __forceinline__ bool find_by_slot(const DecayParams& p, int slot, Segment& g) {
@@ -36,10 +41,10 @@ __device__ __forceinline__ bool find_by_slot(const DecayParams& p, int slot, Seg
   const int i = find_seq_wave(p.qsl, n_live, (int)min(t, (int64_t)INT32_MAX));
   const DecaySeq s = decay_seq(p, i);
   if (s.q_len <= kDecayRows) return false;
-  const int segments = g.segments = (s.q_len + p.seg_len - 1) / p.seg_len;
+  const int segments = g.segments = segments_of(p, s.q_len);
   g.base = s.q0 / p.seg_len;
   g.j = slot - g.base + (AHEAD ? 1 : 0);
-  if (g.j >= segments - (AHEAD ? 0 : 1)) return false;
+  if (segments == 1 || g.j >= segments - (AHEAD ? 0 : 1)) return false;
   g.t0 = s.q0 + g.j * p.seg_len;
   g.n = min(s.q_len - g.j * p.seg_len, p.seg_len);
   g.in = s.in; g.out = s.out;
@@ -63,11 +68,11 @@ __device__ __forceinline__ bool find_segment(const DecayParams& p, int id, Segme
   if (s.q_len <= kDecayRows) return false;
   g.j = 0;
   g.t0 = s.q0;
-  g.n = min(s.q_len, p.seg_len);
+  g.segments = segments_of(p, s.q_len);
+  g.last = g.segments == 1;
+  g.n = g.last ? s.q_len : p.seg_len;
   g.in = s.in; g.out = s.out;
   g.base = s.q0 / p.seg_len;
-  g.segments = (s.q_len + p.seg_len - 1) / p.seg_len;
-  g.last = g.segments == 1;
   return true;
 }
 
@@ -84,32 +89,40 @@ __device__ __forceinline__ int first_key(int direct, int d, int g4) { return dir
 // of several segments may write the slot of the pool it started from while its first segment has yet to run, so the state it
 // starts from is kept too, in a second set of scratch slots.
 __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p) {
+  constexpr int VECS = 2, AHEAD = 4;  // vectors a thread; slots read ahead: the chain is in the sums alone
   Segment g;
   if (!find_by_slot<false>(p, blockIdx.z, g) || g.j != 0) return;
-  const int h = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
-  if (e >= p.scratch_vecs) return;
-  const int lane = e & 63, d = (e >> 6) % p.key_tiles, col = 16 * ((e >> 6) / p.key_tiles) + (lane & 15);
-  const int key = first_key(p.direct, d, lane >> 4);
-  f32x4 r = {};
-  if (g.in >= 0 && col < p.Dv) {
-    const float* from = p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + col;
+  const int h = blockIdx.y, e0 = blockIdx.x * 256 * VECS + threadIdx.x;
+  f32x4 r[VECS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = key + j < p.Dk ? from[(key + j) * p.Dv] : 0.f;
+  for (int v = 0; v < VECS; ++v) {
+    const int e = e0 + v * 256, lane = e & 63, d = (e >> 6) % p.key_tiles, col = 16 * ((e >> 6) / p.key_tiles) + (lane & 15);
+    const int key = first_key(p.direct, d, lane >> 4);
+    r[v] = f32x4{};
+    if (g.in >= 0 && col < p.Dv) {
+      const float* from = p.state + ((int64_t)g.in * p.Hkv + h) * p.Dk * p.Dv + col;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[v][j] = key + j < p.Dk ? from[(key + j) * p.Dv] : 0.f;
+    }
+    scratch_state(p, p.slots + g.base, h)[e] = r[v];
   }
-  scratch_state(p, p.slots + g.base, h)[e] = r;
   const float2 l = decay_power(p.log_decay[h], p.seg_len);
   const int end = g.base + g.segments - 1;
-  constexpr int AHEAD = 4;  // the chain is in the sums alone: the reads of several slots are in flight at once
   for (int slot = g.base; slot < end; slot += AHEAD) {
-    f32x4 a[AHEAD];
+    f32x4 a[AHEAD][VECS];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) a[u] = scratch_state(p, min(slot + u, end - 1), h)[e];
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) a[u][v] = scratch_state(p, min(slot + u, end - 1), h)[e0 + v * 256];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (slot + u >= end) break;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = fmaf(r[j], l.y, fmaf(r[j], l.x, a[u][j]));
-      scratch_state(p, slot + u, h)[e] = r;
+      for (int v = 0; v < VECS; ++v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[v][j] = fmaf(r[v][j], l.y, fmaf(r[v][j], l.x, a[u][v][j]));
+        scratch_state(p, slot + u, h)[e0 + v * 256] = r[v];
+      }
     }
   }
 }
@@ -710,7 +723,7 @@ void launch_tiles(hipStream_t stream, const DecayParams& p) {
   if (p.slots > 0) {
     if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), sums, block, 0, stream, p);
     else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, false>), sums, block, 0, stream, p);
-    hipLaunchKernelGGL(decay_scan_kernel, dim3((p.scratch_vecs + 255) / 256, p.Hkv, p.slots), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3(p.scratch_vecs / 512, p.Hkv, p.slots), dim3(256), 0, stream, p);
   }
   if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, true>), outs, block, 0, stream, p);
   else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, true>), outs, block, 0, stream, p);
