@@ -928,7 +928,8 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
 }
 
 // Segments of the chunked form, from the static bounds: as long as leaves about two workgroups a CU when all T tokens are in
-// use, 256 tokens at the least.  A sequence of up to twice the length that fills the chip is left whole: summing up its first half
+// use; at least 256 tokens, or twice that filling length down to 128 (chains of a few chunks: 64 to 128 tokens of filling length want
+// 256, 47 want 128: the float32 prompts below 58 us against 84).  A sequence of up to twice the length that fills the chip is left whole: summing up its first half
 // ahead costs more than the longer chain.  (48 decode rows beside six prompts of 650 to 2000 tokens, 64 heads of 128 x 128: 196 us
 // whole, 224 us in segments of 1024; one prompt of 16384 tokens of 32 heads: 227 us in segments of 1024, 253 us of 2048.  Where
 // the chip is not filled, short segments pay: four float32 prompts of 450 to 1100 tokens of 8 heads 84 us in segments of 256,
@@ -936,7 +937,7 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
 static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayParams& p, size_t* scratch) {
   const int slices = (Dv + 127) / 128;
   const int64_t cus = std::max(device_cus(), 1);
-  const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus), len = std::max<int64_t>((fill + 63) / 64 * 64, 256);
+  const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus), len = std::max((fill + 63) / 64 * 64, std::min<int64_t>(std::max<int64_t>((2 * fill + 63) / 64 * 64, 128), 256));
   p.seg_len = (int)std::min<int64_t>(len, (int64_t)1 << 30);
   p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, p.seg_len), (int64_t)1 << 30);
   p.slots = T > p.whole_len ? T / p.seg_len + 1 : 0;

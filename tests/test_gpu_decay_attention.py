@@ -162,6 +162,42 @@ def test_in_place_and_step_by_step(gpu, tag):
     assert torch.isfinite(whole).all()
 
 
+@pytest.mark.parametrize("tag", [BF16, F32])
+def test_cut_prompts_in_place(gpu, tag):
+    """Sequences long enough to be cut into segments that run side by side: the slot they start from is the slot they end in."""
+    c = make(51, [1700, 1, 300, 900], Hq=4, Hkv=2, Dk=128, Dv=64, tag=tag, past=[4, 4, 4, 0])
+    d = upload(c, gpu)
+    for _ in range(3):
+        d["state"] = dev(c.state, gpu)
+        out, state = call(d, in_place=True)
+        torch.cuda.synchronize()
+        check(c, out, state, in_place=True)
+
+
+def test_workspace_of_cut_prompts(gpu):
+    """A call that cuts its prompts refuses a workspace below the size it asks for, and needs none where nothing can be cut."""
+    from easydel_amd import _lib
+
+    lib = _lib.load()
+    assert lib.rpa_decay_attention_workspace_bytes(16, 4, 8, 8, 128, 128, 1) == 0
+    need = lib.rpa_decay_attention_workspace_bytes(1700, 1, 4, 2, 128, 64, 1)
+    assert need > 0
+    c = make(52, [1700], Hq=4, Hkv=2, Dk=128, Dv=64)
+    d = upload(c, gpu)
+    out = torch.full((c.T, 4, 64), 7.0, dtype=torch.bfloat16, device=gpu)
+    ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+    args = lambda w, n: (torch.cuda.current_stream().cuda_stream, d["q"].data_ptr(), d["k"].data_ptr(), d["v"].data_ptr(), d["g"].data_ptr(),  # noqa: E731
+                         d["state"].data_ptr(), d["slot_in"].data_ptr(), d["slot_out"].data_ptr(), d["ctx"].data_ptr(), d["qsl"].data_ptr(),
+                         d["ns"].data_ptr(), out.data_ptr(), w, n, c.T, c.S, c.N, 4, 2, 128, 64, 512, 256, 128, 1, 128 ** -0.5)
+    assert lib.rpa_decay_linear_attention(*args(ws.data_ptr(), need - 1)) == _lib.RPA_ERR_WORKSPACE
+    assert lib.rpa_decay_linear_attention(*args(None, need)) == _lib.RPA_ERR_WORKSPACE
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    assert lib.rpa_decay_linear_attention(*args(ws.data_ptr(), need)) == 0
+    torch.cuda.synchronize()
+    check(c, out, d["state"])
+
+
 def test_slots(gpu):
     """Two sequences read one slot (a shared prefix); slots outside the pool read as zeros and are not written."""
     c = make(60, [5, 80, 1, 70], Hq=2, Hkv=2, Dk=64, Dv=64)
