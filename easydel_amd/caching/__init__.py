@@ -1,3 +1,4 @@
+from .decay_state import DecayStateCache, DecayStateCacheConfig, DecayStateCacheView, DecayStateMetadata
 from .metadata_builder import compute_ragged_batch_fields, compute_slot_mapping_v2, request_distribution
 from .ragged_page import (
     RaggedPagesCache,
@@ -12,6 +13,7 @@ from .mla_ragged_page import MLARaggedPagesCache, MLARaggedPagesCacheConfig, MLA
 from .unified_attention import UnifiedAttentionCache, UnifiedAttentionCacheConfig, UnifiedAttentionCacheView
 
 __all__ = [
+    "DecayStateCache", "DecayStateCacheConfig", "DecayStateCacheView", "DecayStateMetadata",
     "MLARaggedPagesCache", "MLARaggedPagesCacheConfig", "MLARaggedPagesCacheView",
     "UnifiedAttentionCache", "UnifiedAttentionCacheConfig", "UnifiedAttentionCacheView",
     "RaggedPagesCache", "RaggedPagesCacheConfig", "RaggedPagesCacheView", "RaggedPagesMetadata", "get_dtype_packing",

@@ -240,6 +240,19 @@ class RaggedPagesCacheView:
         return self
 
 
+    def rope_concatenate_to_cache(self, query, key, value, cache_metadata: RaggedPagesMetadata, rope, positions=None, query_out=None):
+        """Rotates the queries and keys by ``rope`` (an ``operations.Rotary``) and writes keys and values to the positions that
+        the metadata gives the new tokens, in one launch; any page format of the view, scaled pages included.  ``query [T, Hq,
+        D]``, ``key`` / ``value [T, Hkv, D]`` in one 16- or 32-bit type; ``positions [T]`` int32 where the angles go by
+        something else than the cache positions.  Returns the rotated query; the attention that follows reads the pages."""
+        dist = cache_metadata.request_distribution
+        done = kernels.rope_page_scatter_ragged(
+            query, key, value, self.kv_pages, rope.cos_sin, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1),
+            cache_metadata.query_start_loc, cache_metadata.num_seqs.reshape(-1)[:1] if dist is None else dist.reshape(-1)[2:3],
+            kv_scales=self.kv_scales, positions=positions, is_neox_style=rope.is_neox_style, query_out=query_out)
+        return done[0]
+
+
 @dataclass
 class RaggedPagesCache:
     """All layers' views (reference ``RaggedPagesCache.init_cache``, ``cache.py:1040-1100``)."""

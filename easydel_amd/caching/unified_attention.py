@@ -14,6 +14,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from .. import kernels
 from .ragged_page import _BITS, RaggedPagesMetadata, cdiv, kv_cache_update
 
 
@@ -125,6 +126,16 @@ class UnifiedAttentionCacheView:
             kv_cache_update(tokens, cache_metadata.slot_mapping, pool.view(-1, *pool.shape[2:]),
                             cache_metadata.num_kv_update_slices, page_size=int(cache_metadata.page_size))
         return self
+
+    def rope_concatenate_to_cache(self, query, key, value, cache_metadata: RaggedPagesMetadata, rope, positions=None, query_out=None):
+        """Rotates the queries and keys by ``rope`` (an ``operations.Rotary``) and writes keys and values into their pools in one
+        launch, at the positions that lengths, page tables and ``query_start_loc`` give the new tokens (no slot mapping needed).
+        Returns the rotated query."""
+        out, _, _ = kernels.rope_unified_page_scatter(
+            query, key, value, self.key_cache, self.value_cache, rope.cos_sin, cache_metadata.context_lens,
+            cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc, None,  # padded rows have empty spans
+            positions=positions, is_neox_style=rope.is_neox_style, query_out=query_out)
+        return out
 
     def __repr__(self) -> str:
         return (f"{self.__class__.__name__}(layer_index={self.layer_index}, "

@@ -1,7 +1,9 @@
 from ._attention_outputs import AttentionOutput
 from ._base_operation import BaseOperation, EasyDeLBackends, OperationImpl, OperationMetadata, OperationRegistry
+from .decay_linear_attention import DecayLinearAttn
 from .multi_latent_ragged_page_attention import MultiLatentRaggedPageAttn, MultiLatentRaggedPageAttnV2
 from .ragged_page_attention import RaggedPageAttnV2, RaggedPageAttnV3
+from .rotary import Rotary
 from .unified_attention import UnifiedAttn
 from .requirements import (
     CacheRequirements,
@@ -15,6 +17,6 @@ from .requirements import (
 
 __all__ = [
     "AttentionOutput", "BaseOperation", "EasyDeLBackends", "OperationImpl", "OperationMetadata", "OperationRegistry",
-    "RaggedPageAttnV2", "RaggedPageAttnV3", "UnifiedAttn", "MultiLatentRaggedPageAttn", "MultiLatentRaggedPageAttnV2", "CacheRequirements", "CacheType", "ExecutionMode", "MetadataField",
+    "DecayLinearAttn", "RaggedPageAttnV2", "RaggedPageAttnV3", "Rotary", "UnifiedAttn", "MultiLatentRaggedPageAttn", "MultiLatentRaggedPageAttnV2", "CacheRequirements", "CacheType", "ExecutionMode", "MetadataField",
     "MetadataRequirements", "OperationRequirements", "RequirementsBuilder",
 ]

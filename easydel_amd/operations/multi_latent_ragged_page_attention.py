@@ -85,7 +85,7 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
                      softmax_scale: float | None = None, logits_soft_cap: float | None = None,
                      sliding_window: int | None = None, vmem_limit_bytes: int | None = None,
                      mask_value: float | None = None, q_scale: float | None = None, k_scale: float | None = None,
-                     v_scale: float | None = None, softmax_aux=None, **ignore) -> AttentionOutput:
+                     v_scale: float | None = None, softmax_aux=None, rope=None, rope_positions=None, **ignore) -> AttentionOutput:
         name = self.get_impl_name()
         if keys_pe is None:
             raise ValueError(f"{name} requires `keys_pe`. Pass it as `keys_pe=` (or `k_pe=`).")
@@ -116,6 +116,19 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
             raise ValueError("`keys_pe` token dimension must match `queries_nope` token dimension. "
                              f"Got keys_pe={keys_pe.shape[0]} vs queries_nope={queries_nope.shape[0]}.")
         kv_pages = cache_view.kv_pages
+        if rope is not None:
+            # unrotated queries_pe and keys_pe: one launch rotates both and writes the latent rows, then the attention reads
+            distribution = _resolve_distribution(cache_metadata)
+            queries_pe, _ = kernels.rope_mla_page_scatter(
+                queries_pe.to(queries_nope.dtype), keys_values.to(kv_pages.dtype).contiguous(), keys_pe.to(queries_nope.dtype), kv_pages,
+                rope.cos_sin, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc,
+                distribution[2:3], positions=rope_positions, is_neox_style=rope.is_neox_style)
+            output, _ = kernels.mla_ragged_paged_attention(
+                queries_nope.contiguous(), queries_pe, None, None, kv_pages, cache_metadata.context_lens,
+                cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc,
+                torch.stack([torch.zeros_like(distribution[2]), torch.zeros_like(distribution[2]), distribution[2]]),
+                softmax_scale=softmax_scale, sliding_window=sliding_window, logits_soft_cap=logits_soft_cap, softmax_aux=softmax_aux)
+            return AttentionOutput(attention_weights=None, attention_outputs=output.reshape(shape4) if is_4d else output, cache_view=cache_view)
         if keys_values.dtype != kv_pages.dtype or keys_pe.dtype != kv_pages.dtype:
             if kv_pages.element_size() < max(keys_values.element_size(), keys_pe.element_size()):
                 logger.warning("Casting keys_values/keys_pe from %s to lower-precision KV cache dtype %s; "
@@ -138,13 +151,15 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
     def forward_core_dp_local_shard(self, queries_nope, queries_pe, keys_values, keys_pe, local_kv_pages, cache_metadata,
                                     shard_index: int, num_shards: int, softmax_scale: float | None = None,
                                     logits_soft_cap: float | None = None, sliding_window: int | None = None,
-                                    softmax_aux=None, **ignore):
+                                    softmax_aux=None, rope=None, **ignore):
         """One data-parallel rank's share when the latent pages are sharded over ranks and every sequence's pages live
         on the rank of its metadata row (the body of the reference's ``shard_map`` at :507-566, before the sum over
         ranks): metadata rows sliced, page ids rebased and clipped, distribution recomputed, fused write + attention on
         the rank's pages; the rows of other ranks' tokens come back as zeros.  Operands already flattened
         (``[tokens, heads, dim]`` / ``[tokens, dim]``) and in the page dtype.  Returns ``(local_output, local_kv_pages)``;
         the ranks' outputs are summed in float32 (``ragged_page_attention.dp_local_reduce``)."""
+        if rope is not None:
+            raise NotImplementedError("the shard-local form takes rotated queries and keys (kernels.rope_mla_page_scatter writes a rank's pages)")
         from .ragged_page_attention import dp_local_metadata
 
         context_lens, tables, query_start_loc, distribution = dp_local_metadata(cache_metadata, shard_index, num_shards,

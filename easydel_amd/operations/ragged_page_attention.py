@@ -7,6 +7,10 @@ the cache dtype with a warning when it narrows (:570-580), write-back of the upd
 (:747), ``softmax_aux`` attention sinks (one logit per query head, cast to float32 as at :469-471) and
 ``AttentionOutput`` result.  Where the reference hands the arrays to ``ejkernel`` (:281-313,
 :732-746), this module hands device pointers to ``librpa_hip.so`` through ``easydel_amd.kernels``.
+
+``rope=`` (an ``operations.Rotary``), an addition to the reference's signature, hands the v3 operation queries and keys that
+are not rotated yet: the page write rotates them on the way (``rope_positions [T]`` where the angles go by something else than
+the cache positions).
 """
 
 from __future__ import annotations
@@ -68,7 +72,9 @@ class _RaggedPageAttn(OperationImpl):
     def forward_v2(self, query, cache_view: RaggedPagesCacheView, cache_metadata: RaggedPagesMetadata,
                    softmax_scale: float | None = None, logits_soft_cap: float | None = None, compute_dtype=None,
                    optimized: bool = False, sliding_window: int | None = None, softmax_aux=None,
-                   mask_value: float | None = None, vmem_limit_bytes: int | None = None, **ignore) -> AttentionOutput:
+                   mask_value: float | None = None, vmem_limit_bytes: int | None = None, rope=None, **ignore) -> AttentionOutput:
+        if rope is not None:
+            raise NotImplementedError("ragged_page_attention_v2 only reads the pages: rotate with the view's `rope_concatenate_to_cache`")
         output = kernels.ragged_paged_attention(
             query, cache_view.kv_pages, cache_metadata.context_lens, cache_metadata.pages_tables,
             cache_metadata.query_start_loc, cache_metadata.num_seqs.reshape(-1), softmax_scale=softmax_scale,
@@ -80,8 +86,20 @@ class _RaggedPageAttn(OperationImpl):
     # -- v3: fused page write + attention ------------------------------------------------------------------
     def forward_v3(self, query, key, value, cache_view: RaggedPagesCacheView, cache_metadata: RaggedPagesMetadata,
                    softmax_scale: float | None = None, logits_soft_cap: float | None = None,
-                   sliding_window: int | None = None, softmax_aux=None, **ignore) -> AttentionOutput:
+                   sliding_window: int | None = None, softmax_aux=None, rope=None, rope_positions=None, **ignore) -> AttentionOutput:
         kv_pages = cache_view.kv_pages
+        if rope is not None:
+            # unrotated queries and keys: one launch rotates both, writes the pages (coding them where they are scaled), then
+            # the attention reads
+            if key is None or value is None:
+                raise ValueError("ragged_page_attention_v3 with `rope` needs the step's key and value")
+            query = cache_view.rope_concatenate_to_cache(query, key, value, cache_metadata, rope, positions=rope_positions)
+            output = kernels.ragged_paged_attention(
+                query, kv_pages, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1),
+                cache_metadata.query_start_loc, cache_metadata.request_distribution[2:3], softmax_scale=softmax_scale,
+                sliding_window=sliding_window, logits_soft_cap=logits_soft_cap, kv_scales=getattr(cache_view, "kv_scales", None),
+                num_kv_heads=key.shape[1], softmax_aux=softmax_aux)
+            return AttentionOutput(attention_weights=None, attention_outputs=output, cache_view=cache_view)
         if getattr(cache_view, "kv_scales", None) is not None:
             # scaled 8-bit pages: the write quantises (per page and head the scale only grows), then the attention
             # reads codes and scales
@@ -119,7 +137,7 @@ class _RaggedPageAttn(OperationImpl):
     def forward_v3_dp_local_shard(self, query, key, value, local_kv_pages, cache_metadata: RaggedPagesMetadata,
                                   shard_index: int, num_shards: int, softmax_scale: float | None = None,
                                   logits_soft_cap: float | None = None, sliding_window: int | None = None,
-                                  softmax_aux=None, local_kv_scales=None, num_kv_heads: int | None = None, **ignore):
+                                  softmax_aux=None, local_kv_scales=None, num_kv_heads: int | None = None, rope=None, **ignore):
         """What one data-parallel rank computes when the page pool is sharded over ranks and every sequence's pages
         live on the rank that owns its metadata row (the body of the reference's ``shard_map`` at :645-717, before the
         sum over ranks): the rank takes its ``S / num_shards`` rows of ``context_lens``, ``pages_tables`` and
@@ -133,6 +151,8 @@ class _RaggedPageAttn(OperationImpl):
         A rank's share of a scaled 8-bit pool comes with its rows of the scales, ``local_kv_scales [local_pages, C]``:
         the write then quantises and the call returns ``(local_output, local_kv_pages, local_kv_scales)``.  int8 pages
         without scales are refused (only fp8 pages may hold bare codes, the reference's cast-only cache)."""
+        if rope is not None:
+            raise NotImplementedError("the shard-local form takes rotated queries and keys (kernels.rope_page_scatter_ragged writes a rank's pages)")
         context_lens, tables, query_start_loc, distribution = dp_local_metadata(cache_metadata, shard_index, num_shards, int(local_kv_pages.shape[0]))
         if local_kv_scales is not None:
             if key.dtype not in (torch.float32, torch.bfloat16):
@@ -173,7 +193,9 @@ class _RaggedPageAttn(OperationImpl):
                  vmem_limit_bytes: int | None = None, **ignore) -> AttentionOutput:
         is_4d = query.ndim == 4
         shape4 = tuple(query.shape) if is_4d else None
-        query_r = query.reshape(-1, *query.shape[-2:]).contiguous()
+        query_r = query.reshape(-1, *query.shape[-2:])
+        if ignore.get("rope") is None:  # the rotating write reads views of a projection as they are
+            query_r = query_r.contiguous()
         key_r = None if key is None else key.reshape(-1, *key.shape[-2:])
         value_r = None if value is None else value.reshape(-1, *value.shape[-2:])
         output = super().__call__(query=query_r, key=key_r, value=value_r, cache_view=cache_view,

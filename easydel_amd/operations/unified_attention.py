@@ -39,7 +39,9 @@ class UnifiedAttn(OperationImpl):
 
     def forward_native(self, query, cache_view: UnifiedAttentionCacheView | None, cache_metadata: RaggedPagesMetadata,
                        softmax_scale: float | None = None, causal: bool = True, sliding_window: int | None = None,
-                       logits_soft_cap: float | None = None, softmax_aux=None, **ignore) -> AttentionOutput:
+                       logits_soft_cap: float | None = None, softmax_aux=None, rope=None, **ignore) -> AttentionOutput:
+        if rope is not None:
+            raise NotImplementedError("unified_attention only reads the pools: rotate with the view's `rope_concatenate_to_cache`")
         if cache_view is None:
             raise ValueError("UnifiedAttn requires `cache_view` (paged KV cache).")
         if not causal:
