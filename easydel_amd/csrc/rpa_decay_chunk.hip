@@ -380,8 +380,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_k
     for (int gq = 0; gq < groups; ++gq) {
       const int step = c * groups + gq;
       // this step's tiles have arrived, and the other buffers have been read.  Behind the tiles' loads this wave issued the two
-      // stores of the step before where it holds 16 columns (`whole`): they need not be waited for.
-      if (whole && step > 0) wait_loads<2>();
+      // stores of the step before, which need not be waited for, if it holds 16 columns (`whole`) and that step's chunk was full:
+      // the chunks before this one are, and this one is if it has kChunk tokens.  In a part of a chunk a wave without rows to write
+      // issues fewer stores, and a wait for two outstanding operations would let the tile itself be one of them.
+      if (whole && step > 0 && (gq == 0 || n == kChunk)) wait_loads<2>();
       else wait_loads<0>();
       __syncthreads();
       const bool on = gq == groups - 1;  // the next step is another chunk's

@@ -162,6 +162,22 @@ def test_in_place_and_step_by_step(gpu, tag):
     assert torch.isfinite(whole).all()
 
 
+@pytest.mark.parametrize("group", [2, 4, 7])
+@pytest.mark.parametrize("tail", [1, 5, 16, 17, 31])
+def test_last_chunks_of_shared_heads(gpu, group, tail):
+    """Several query heads a KV head in a last chunk that is not full: each head's queries are waited for although the stores of the
+    head before were fewer.  Many sequences, so that the loads are slow."""
+    c = make(54 + tail, [32 + tail] * 64, Hq=2 * group, Hkv=2, Dk=128, Dv=128)
+    d = upload(c, gpu)
+    out, state = call(d)
+    out, state = out.clone(), state.clone()
+    check(c, out, state)
+    for _ in range(5):
+        again, _ = call(d)
+        torch.cuda.synchronize()
+        assert torch.equal(out, again) and torch.equal(state, d["state"])
+
+
 @pytest.mark.parametrize("tag", [BF16, F32])
 def test_cut_prompts_in_place(gpu, tag):
     """Sequences long enough to be cut into segments that run side by side: the slot they start from is the slot they end in."""
