@@ -993,7 +993,7 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
   p.rows = T;
   hipStream_t s = (hipStream_t)stream;
   // (rows that lie 2^23 elements apart would pass the chunked form's 32-bit offsets in a chunk: the recurrent form takes them)
-  const bool near = std::max(query_stride, std::max(key_stride, value_stride)) < ((int64_t)1 << 23);
+  const bool near = std::max(std::max(query_stride, (int64_t)Hq * Dv), std::max(key_stride, value_stride)) < ((int64_t)1 << 23);
   if (T > rpa::kDecayRows && near) {
     size_t scratch;
     decay_segments(T, S, Hkv, Dk, Dv, p, &scratch);

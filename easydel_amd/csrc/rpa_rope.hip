@@ -262,7 +262,7 @@ __device__ __forceinline__ void append_run(const RopeParams& p, int n_live, int 
   const int i = find_run_wave(p.qsl, n_live, p.page_size, run);
   const int q0 = p.qsl[i], q_len = p.qsl[i + 1] - q0;
   const int ctx = p.context_lens[i];
-  if (q_len <= 0) return;
+  if (q_len <= 0 || q0 < 0) return;
   const int pos0 = max(ctx - q_len, 0);                        // first position written
   const int j = pos0 / p.page_size + (run - (q0 / p.page_size + 2 * i));
   const int64_t begin = (int64_t)j * p.page_size;              // first position of the page

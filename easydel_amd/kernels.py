@@ -638,7 +638,8 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
     [T, Hq, Dk]``, ``key [T, Hkv, Dk]``, ``value [T, Hkv, Dv]`` of one dtype (float32, bfloat16, float16; token rows may lie
     apart) and ``state [slots, Hkv, Dk, Dv]`` float32, one state to ``Hq / Hkv`` query heads.  Sequence ``i`` goes on from slot
     ``state_indices[i]``, or from zero where ``context_lens[i]`` says that it has no tokens before these, and leaves its
-    state in ``state_out_indices[i]`` (default: the same slot).  ``scale`` defaults to ``Dk ** -0.5``.  Returns ``(out [T, Hq,
+    state in ``state_out_indices[i]`` (default: the same slot); slots written must differ from each other and from those that other
+    sequences of the call read.  ``scale`` defaults to ``Dk ** -0.5``.  Returns ``(out [T, Hq,
     Dv], state)``: the pool updated in place, rows of padded tokens zeros."""
     lib = _lib.load()
     if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:

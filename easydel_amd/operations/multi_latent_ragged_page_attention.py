@@ -120,7 +120,7 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
             # unrotated queries_pe and keys_pe: one launch rotates both and writes the latent rows, then the attention reads
             distribution = _resolve_distribution(cache_metadata)
             queries_pe, _ = kernels.rope_mla_page_scatter(
-                queries_pe.to(queries_nope.dtype), keys_values.to(kv_pages.dtype).contiguous(), keys_pe.to(queries_nope.dtype), kv_pages,
+                queries_pe, keys_values.to(kv_pages.dtype).contiguous(), keys_pe, kv_pages,  # (both of one type: rounding ahead of the rotation is the caller's)
                 rope.cos_sin, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc,
                 distribution[2:3], positions=rope_positions, is_neox_style=rope.is_neox_style)
             output, _ = kernels.mla_ragged_paged_attention(

@@ -62,7 +62,7 @@ class UnifiedAttn(OperationImpl):
     def forward_dp_local_shard(self, query, local_key_cache, local_value_cache, cache_metadata: RaggedPagesMetadata,
                                shard_index: int, num_shards: int, softmax_scale: float | None = None,
                                sliding_window: int | None = None, logits_soft_cap: float | None = None, softmax_aux=None,
-                               **ignore):
+                               rope=None, **ignore):
         """What one data-parallel rank computes when the K and V pools are sharded over ranks and every sequence's pages
         live on the rank of its metadata row (the body of the reference's ``shard_map`` at :296-353, before the sum over
         ranks): its rows of the lengths, page tables and ``query_start_loc``, page ids rebased by
@@ -70,6 +70,8 @@ class UnifiedAttn(OperationImpl):
         index 0 (its kernel needs ``query_start_loc[0] == 0``, :319-327) and zeroes the other ranks' tokens afterwards
         (:345-353); these kernels take the global token indices as they are and write zeros for tokens outside the
         rank's span, so neither step exists here.  ``query`` is ``[tokens, heads, dim]``; returns the local output."""
+        if rope is not None:
+            raise NotImplementedError("the shard-local form takes rotated queries (kernels.rope_unified_page_scatter writes a rank's pools)")
         S = int(cache_metadata.context_lens.shape[0])
         if num_shards <= 0 or S % num_shards != 0:
             raise ValueError(f"{S} metadata rows do not divide over {num_shards} shards")

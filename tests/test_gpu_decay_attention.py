@@ -339,3 +339,82 @@ def test_random_batches(gpu):
         out, state = call(d)
         torch.cuda.synchronize()
         check(c, out, state)
+
+
+@pytest.mark.parametrize("tag", [BF16, F32])
+def test_many_padded_rows(gpu, tag):
+    """More metadata rows than the tokens could fill: segments are numbered by token instead of by row."""
+    for lens, pad in (([17, 1, 0, 40, 18], 300), ([90], 200), ([700, 2, 33], 4000), ([1, 2], 64)):
+        c = make(70, lens, Hq=4, Hkv=2, Dk=64, Dv=64, tag=tag, pad_rows=pad, pad_tokens=3, slots=2 * len(lens) + 2, past=[2] * len(lens))
+        c.slot_in[:len(lens)] = np.arange(len(lens))
+        c.slot_out[:len(lens)] = len(lens) + np.arange(len(lens))
+        d = upload(c, gpu)
+        out, state = call(d)
+        torch.cuda.synchronize()
+        check(c, out, state)
+        assert not out[int(c.qsl[c.n]):].any()
+
+
+def test_one_graph_serves_other_batches_of_its_bounds(gpu):
+    """Lengths, slots and live rows are read by the kernels: a graph captured over one batch is replayed over others."""
+    first = make(71, [600, 1, 40, 30], Hq=4, Hkv=2, Dk=128, Dv=128)
+    d = upload(first, gpu)
+    out = torch.empty((first.T, 4, 128), dtype=torch.bfloat16, device=gpu)
+    call(d, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(d, out=out)
+    for seed, lens, pad_rows in ((72, [1, 1, 1, 1], 0), (73, [671], 3), (74, [16, 17, 300, 0], 0), (75, [5, 650], 2), (71, [600, 1, 40, 30], 0)):
+        c = make(seed, lens, Hq=4, Hkv=2, Dk=128, Dv=128, pad_rows=pad_rows, pad_tokens=first.T - sum(lens))
+        for key, new in upload(c, gpu).items():
+            d[key].copy_(new)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(c, out, d["state"])
+        assert not out[int(c.qsl[c.n]):].any()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams have scratch of their own."""
+    cases = [make(76 + i, [1500, 3, 200], Hq=4, Hkv=2, Dk=128, Dv=128) for i in range(2)]
+    data = [upload(c, gpu) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        for c, d in zip(cases, data):
+            d["state"].copy_(dev(c.state, gpu))
+        torch.cuda.synchronize()
+        outs = []
+        for d, s in zip(data, streams):
+            with torch.cuda.stream(s):
+                outs.append(call(d)[0])
+        torch.cuda.synchronize()
+        for c, d, out in zip(cases, data, outs):
+            check(c, out, d["state"])
+
+
+def test_rows_far_apart(gpu):
+    """Token rows 2^23 elements apart: offsets inside a chunk pass 31 bits."""
+    c = make(79, [40, 3], Hq=1, Hkv=1, Dk=16, Dv=16)
+    d = upload(c, gpu)
+    wide = torch.zeros((c.T, 1 << 23), dtype=torch.bfloat16, device=gpu)
+    for name, at in (("q", 0), ("k", 16), ("v", 32)):
+        wide[:, at:at + 16] = d[name].flatten(1)
+        d[name] = wide[:, at:at + 16].unflatten(1, (1, 16))
+    out, state = call(d)
+    torch.cuda.synchronize()
+    check(c, out, state)
+
+
+def test_no_tokens(gpu):
+    c = make(80, [4], Hq=2, Hkv=2)
+    d = upload(c, gpu)
+    want = d["state"].clone()
+    empty = dict(d, q=d["q"][:0], k=d["k"][:0], v=d["v"][:0])
+    out, state = call(empty)
+    assert tuple(out.shape) == (0, 2, 64) and torch.equal(state, want)
+    d["ns"].zero_()
+    out, state = call(d)  # no live row: outputs are zeros, states as they were
+    torch.cuda.synchronize()
+    assert not out.any() and torch.equal(state, want)

@@ -67,3 +67,6 @@ def test_reading_operations_refuse_a_rotation():
     with pytest.raises(NotImplementedError, match="shard-local"):
         meta = RaggedPagesMetadata.create_empty(1, 1, 1, version="v3", device="cpu")
         op.forward_v3_dp_local_shard(q, q, q, torch.zeros(1, 16, 2, 8), meta, 0, 1, rope=r)
+    with pytest.raises(NotImplementedError, match="shard-local"):
+        pool = torch.zeros(1, 16, 1, 8)
+        OperationRegistry.create("unified_attention", OperationMetadata()).forward_dp_local_shard(q, pool, pool, meta, 0, 1, rope=r)
