@@ -939,7 +939,7 @@ static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayPara
   const int64_t cus = std::max(device_cus(), 1);
   const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus), len = std::max((fill + 63) / 64 * 64, std::min<int64_t>(std::max<int64_t>((2 * fill + 63) / 64 * 64, 128), 256));
   p.seg_len = (int)std::min<int64_t>(len, (int64_t)1 << 30);
-  p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, p.seg_len), (int64_t)1 << 30);
+  p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, std::max(p.seg_len, 256)), (int64_t)1 << 30);
   p.slots = T > p.whole_len ? T / p.seg_len + 1 : 0;
   const int by_token = T / (rpa::kDecayRows + 1) + 1;
   p.first_by_seq = S <= by_token;
@@ -1003,9 +1003,9 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
     p.vec = ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)value)) & 15) == 0 && query_stride % unit == 0 && key_stride % unit == 0 &&
             value_stride % unit == 0 && Dk % unit == 0 && Dv % unit == 0;
     p.direct = dtype == RPA_BF16 && p.vec;
-    const int64_t blocks = ((int64_t)p.first_ids + p.slots) * Hkv * 4;
+    const int64_t blocks = ((int64_t)p.first_ids + p.slots + S + 64) * Hkv * 4;
     if (blocks > INT32_MAX || p.slots > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: T=%d tokens of %d heads are too many workgroups", who, T, Hkv);
-    if (const int err = rpa::launch_decay_chunk(s, p)) return hip_fail(err, "rpa_decay_linear_attention chunk launch");
+    return hip_fail(rpa::launch_decay_chunk(s, p), "rpa_decay_linear_attention chunk launch");
   }
   return hip_fail(rpa::launch_decay_recurrent(s, p), "rpa_decay_linear_attention launch");
 }

@@ -28,6 +28,7 @@ struct DecayParams {
   int slots;         // scratch slots: floor(T / seg_len) + 1, 0 where no sequence can be cut
   int first_ids;     // numbers that first segments may have ...
   int first_by_seq;  // ... which are their sequences' (1) or floor(qsl[i] / (kDecayRows + 1)) (0)
+  int chunk_blocks;  // workgroups of the chunked form, ahead of those of the recurrent one in the same launch
   int direct;        // the bf16 kernel serves the call (the float32 one otherwise): the order of a scratch state's keys
   int key_tiles;     // tiles of 16 keys the kernels compute with (4, 8 or 16)
   int scratch_vecs;  // 16-byte vectors of a scratch state: columns and keys padded to what the kernels compute with

@@ -11,12 +11,14 @@
 // launched where the bounds allow a sequence of more than one segment.  The first segments are numbered by sequence or by
 // floor(qsl[i] / (kDecayRows + 1)), the others by floor(qsl[i] / seg_len) + j - 1: both are distinct without a plan, since such
 // a sequence is longer than the divisor.
-#include "rpa_decay.h"
+#include "rpa_decay_steps.h"
 #include "rpa_mfma.h"
 
 namespace rpa {
 
 namespace {
+
+constexpr int kClearBlocks = 64;
 
 struct Segment {
   int j, t0, n;      // segment of its sequence, first token, tokens
@@ -79,6 +81,19 @@ __device__ __forceinline__ bool find_segment(const DecayParams& p, int id, Segme
 // A scratch state lies as the lanes of the chunk kernels hold it, 16 bytes a lane and tile of 16 keys: [16-column group][tile][lane].
 __device__ __forceinline__ f32x4* scratch_state(const DecayParams& p, int slot, int h) {
   return (f32x4*)p.scratch + ((int64_t)slot * p.Hkv + h) * p.scratch_vecs;
+}
+
+// Workgroups behind the chunked form's own take the sequences of few tokens, then the padded rows: the chains of chunks leave HBM
+// room that the states of decode rows use.  (48 decode rows beside six prompts of 650 to 2000 tokens, 64 heads of 128 x 128: 222 us;
+// a launch of its own for the decode rows 190 + 65 us.  256 decode rows alone: 370 us, 5.8 TB/s, against 385 + 6 us.)
+template <int DT, int DK, int NW>
+__device__ __forceinline__ void beside_chunks(const DecayParams& p, int id, int heads, int slices, char* lds) {
+  if (id >= p.S * heads) {
+    clear_padded_rows<DT>(p, id - p.S * heads, kClearBlocks);
+    return;
+  }
+  const int i = id / heads, hs = id - i * heads, h = hs / slices;
+  decay_steps<DT, 64 * NW, 4 * NW, DK / 16>(p, i, h, (hs - h * slices) * 16 * NW, *(StepLds<64 * NW, 4 * NW>*)lds);
 }
 
 // The first of the four keys that a lane group holds of tile d: in the order in which the bf16 kernel reads the queries, or as they
@@ -328,6 +343,13 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_k
 
   const int slices = (p.Dv + DV - 1) / DV, heads = p.Hkv * slices;
   const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
+  if constexpr (OUT) {
+    static_assert(sizeof(sK) >= sizeof(StepLds<NT, 4 * NW>), "the short sequences' work uses the tiles' memory");
+    if ((int)blockIdx.x >= p.chunk_blocks) {
+      beside_chunks<RPA_BF16, DK, NW>(p, blockIdx.x - p.chunk_blocks, heads, slices, (char*)sK);
+      return;
+    }
+  }
   Segment g;
   if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, i16 = lane & 15, g4 = lane >> 4;
@@ -565,6 +587,13 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
 
   const int slices = (p.Dv + DV - 1) / DV, heads = p.Hkv * slices;
   const int id = blockIdx.x / heads, hs = blockIdx.x - id * heads, h = hs / slices, c0 = (hs - h * slices) * DV;
+  if constexpr (OUT) {
+    static_assert(sizeof(sK) >= sizeof(StepLds<NT, 4 * NW>), "the short sequences' work uses the tiles' memory");
+    if ((int)blockIdx.x >= p.chunk_blocks) {
+      beside_chunks<DT, DK, NW>(p, blockIdx.x - p.chunk_blocks, heads, slices, (char*)sK);
+      return;
+    }
+  }
   Segment g;
   if (OUT ? !find_segment(p, id, g) : !find_by_slot<false>(p, id, g)) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, i16 = lane & 15, g4 = lane >> 4;
@@ -719,9 +748,10 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
 // Rows of 16-byte aligned bf16 take the bf16 kernel, everything else the float32 one; eight waves (128 columns) a workgroup, four
 // where the values have at most 64.
 template <int DT, int DK, int NW, bool DIRECT>
-void launch_tiles(hipStream_t stream, const DecayParams& p) {
+void launch_tiles(hipStream_t stream, DecayParams p) {
   const int slices = (p.Dv + 16 * NW - 1) / (16 * NW), heads = p.Hkv * slices;
-  const dim3 block(64 * NW), sums(p.slots * heads), outs((p.first_ids + p.slots) * heads);
+  p.chunk_blocks = (p.first_ids + p.slots) * heads;
+  const dim3 block(64 * NW), sums(p.slots * heads), outs(p.chunk_blocks + p.S * heads + kClearBlocks);
   if (p.slots > 0) {
     if constexpr (DIRECT) hipLaunchKernelGGL((decay_chunk_bf16_kernel<DK, NW, false>), sums, block, 0, stream, p);
     else hipLaunchKernelGGL((decay_chunk_wide_kernel<DT, DK, NW, false>), sums, block, 0, stream, p);
