@@ -928,16 +928,19 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
 }
 
 // Segments of the chunked form, from the static bounds: as long as leaves about two workgroups a CU when all T tokens are in
-// use; at least 256 tokens, or twice that filling length down to 128 (chains of a few chunks: 64 to 128 tokens of filling length want
-// 256, 47 want 128: the float32 prompts below 58 us against 84).  A sequence of up to twice the length that fills the chip is left whole: summing up its first half
-// ahead costs more than the longer chain.  (48 decode rows beside six prompts of 650 to 2000 tokens, 64 heads of 128 x 128: 196 us
-// whole, 224 us in segments of 1024; one prompt of 16384 tokens of 32 heads: 227 us in segments of 1024, 253 us of 2048.  Where
-// the chip is not filled, short segments pay: four float32 prompts of 450 to 1100 tokens of 8 heads 84 us in segments of 256,
-// 137 us with sequences of up to 512 left whole.)  scratch: bytes of the states between segments.
+// use; where that fills the chip with less than 256 tokens each, up to twice that and at least 64, for the chain of chunks is
+// what such calls wait for.  (One prompt of 16384 tokens of 32 heads: 227 us in segments of 1024, 253 us of 2048.  One of 1000
+// tokens, float32, 2 heads: 34 us in segments of 64, 49 us of 128; one of 6000 bfloat16 tokens of 16 heads 53 us in segments of twice
+// the filling length, 62 us of just that.)
+// A sequence of up to twice the length that fills the chip is left whole: summing up its first half ahead costs more than the
+// longer chain (48 decode rows beside six prompts of 650 to 2000 tokens, 64 heads of 128 x 128: 196 us whole, 224 us in segments
+// of 1024); so is one of up to 256 tokens, whose few chunks cost what two more launches do.
+// scratch: bytes of the states between segments.
 static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayParams& p, size_t* scratch) {
   const int slices = (Dv + 127) / 128;
   const int64_t cus = std::max(device_cus(), 1);
-  const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus), len = std::max((fill + 63) / 64 * 64, std::min<int64_t>(std::max<int64_t>((2 * fill + 63) / 64 * 64, 128), 256));
+  const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus);
+  const int64_t len = std::max((fill + 63) / 64 * 64, std::min<int64_t>((2 * fill + 63) / 64 * 64, 256));
   p.seg_len = (int)std::min<int64_t>(len, (int64_t)1 << 30);
   p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, std::max(p.seg_len, 256)), (int64_t)1 << 30);
   p.slots = T > p.whole_len ? T / p.seg_len + 1 : 0;

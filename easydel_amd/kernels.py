@@ -434,7 +434,7 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device) 
     # what a good call looks like first, in few steps: a decode step's launch waits for them
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.shape == shape:
         if t.is_contiguous():
-            return t.data_ptr(), math.prod(shape[1:])
+            return t.data_ptr(), shape[1] * shape[2] if len(shape) == 3 else shape[1]
         st = t.stride()
         if len(st) == 3 and st[2] == 1 and st[1] == shape[2] and shape[0] > 1:
             return t.data_ptr(), st[0]
@@ -461,7 +461,7 @@ def _launch(device, fn, *args) -> None:
     launches on that)."""
     index = device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:  # a tensor of the device exists: the runtime is initialised
         code = fn(stream, *args)
     else:
         with torch.cuda.device(device):
@@ -683,8 +683,10 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
     if T > 0:
         tag = _DTYPE_TAG[dt]
         # scratch of its own for every call: the caching allocator orders its reuse by stream, and a captured graph keeps its own
-        with torch.cuda.device(dev):  # the size goes by the current device's compute units
-            need = lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, tag) if T > 1 else 0
+        need = 0
+        if T > 256:  # nothing is cut below that
+            with torch.cuda.device(dev):  # the size goes by the current device's compute units
+                need = lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, tag)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _launch(dev, lib.rpa_decay_linear_attention, q, k, v, *ptrs, o, None if ws is None else ws.data_ptr(), need, T, S, state.shape[0],
                 Hq, Hkv, Dk, Dv, qs, ks, vs, tag, float(Dk) ** -0.5 if scale is None else float(scale))
