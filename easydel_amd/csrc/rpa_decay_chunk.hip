@@ -85,7 +85,7 @@ __device__ __forceinline__ f32x4* scratch_state(const DecayParams& p, int slot, 
 
 // Workgroups behind the chunked form's own take the sequences of few tokens, then the padded rows: the chains of chunks leave HBM
 // room that the states of decode rows use.  (48 decode rows beside six prompts of 650 to 2000 tokens, 64 heads of 128 x 128: 222 us;
-// a launch of its own for the decode rows 190 + 65 us.  256 decode rows alone: 370 us, 5.8 TB/s, against 385 + 6 us.)
+// a launch of its own for the decode rows 190 + 65 us.  256 decode rows alone: 358 to 370 us, 5.8 to 6.0 TB/s, against 385 + 6 us.)
 template <int DT, int DK, int NW>
 __device__ __forceinline__ void beside_chunks(const DecayParams& p, int id, int heads, int slices, char* lds) {
   if (id >= p.S * heads) {
@@ -199,18 +199,24 @@ __device__ __forceinline__ void store_state(const DecayParams& p, const Segment&
 // Rounded to bf16 are the scores and, for the product with the queries only, the state: what they add to an output is rounded
 // to bf16 as well.  The tiles of the next chunk are on their way into LDS (direct loads, two buffers) while this one is worked on.
 // What a chunk costs is mostly the latency of its chain (tiles, scores, barrier, products, store); sixteen waves a CU with 16
-// columns each hide it better than eight with 32.
+// columns each hide it better than eight with 32 (152 against 127 us below).
+// Measured: one prompt of 16384 tokens, 32 heads of 128 x 128: sums 70 us (268 MB, 3.8 TB/s), scan 14 us, outputs 126 to 146 us (537 MB,
+// 3.7 to 4.3 TB/s).  In a round of two workgroups a CU (9400 cycles) the matrix units work for 2400 cycles, LDS for
+// 2300, the vector units for 3900, one after the other more than side by side.
 
 constexpr int kChunk = 32;
 constexpr int kScoreRow = 80;  // bytes of a row of 32 bf16 scores in LDS, spread over the banks
 
-// 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key: sixteen consecutive rows read at one chunk, and four
-// rows read by the transposing loads at a pair or an aligned group of four chunks, fall on distinct banks (a row of 128 elements
-// spans all of them, one of 64 half).
+// 16-byte chunks of a row of WIDTH elements are stored XOR-ed with this key.  LDS serves a 16-byte read in groups of sixteen lanes that
+// take rows 0-3 and 12-15 from one lane group and rows 4-11 from its neighbour, whose chunk differs in the lowest bit: with the
+// last two bits of the key counting down over the quads of rows, all sixteen fall on distinct banks (counting up, pairs
+// collide: 30 % more LDS cycles, the segments of five prompts of 1200 tokens of 16 heads 162 instead of 158 us a call).  The transposing reads of a pair of chunks find theirs distinct as well; those of four
+// chunks (the keys) read one half of each and meet the same banks twice whatever the key.
 template <int WIDTH>
 __device__ __forceinline__ int tile_key(int row) {
-  if constexpr (WIDTH >= 128) return ((row & 3) << 2) | ((row >> 2) & 3);
-  else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  const int down = -(row >> 2) & 3;
+  if constexpr (WIDTH >= 128) return ((row & 3) << 2) | down;
+  else return (((row >> 1) & 1) << 2) | down;  // (128-byte rows: their lowest bit chooses half of the banks)
 }
 
 typedef __attribute__((address_space(3))) const char lds_char;
@@ -527,7 +533,9 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_k
 // The same chunks, tiles and owners with 16 x 16 x 4 float32 instructions (a sixteenth of the bf16 rate), elements widened to
 // float32 on their way into LDS.  Nothing is rounded on the way, and any row the checks allow can be read; the tiles of the next
 // chunk wait in registers (six pieces of four elements a thread at 128 keys).  Lane (i, g), register j of tile d of the state: key
-// 16 d + 4 g + j of column i.
+// 16 d + 4 g + j of column i.  Measured: four float32 prompts of 450 to 1100 tokens, 16 + 8 heads of 64 x 96: sums 12.6 us, scan 7.6 us,
+// outputs 34 us: chains of four chunks of two query heads, 8000 cycles of matrix instructions in each at the two waves that
+// share a SIMD.
 constexpr int kWidePad = 4;  // floats behind a row of LDS: rows start four banks apart
 
 template <int DT>

@@ -9,7 +9,7 @@
 namespace rpa {
 
 // A state is next wanted a whole model's worth of traffic later: past the caches, reads and writes stream faster (256 states of 64
-// heads of 128 x 128: 393 -> 374 us, 5.8 TB/s).
+// heads of 128 x 128: 393 -> 374 us).
 __device__ __forceinline__ float4 load_once(const float* at) {
   typedef float f4 __attribute__((ext_vector_type(4)));
   const f4 x = __builtin_nontemporal_load((const f4*)at);
