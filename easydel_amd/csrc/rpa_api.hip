@@ -1006,8 +1006,10 @@ int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const voi
     p.vec = ((((uintptr_t)query) | ((uintptr_t)key) | ((uintptr_t)value)) & 15) == 0 && query_stride % unit == 0 && key_stride % unit == 0 &&
             value_stride % unit == 0 && Dk % unit == 0 && Dv % unit == 0;
     p.direct = dtype == RPA_BF16 && p.vec;
-    const int64_t blocks = ((int64_t)p.first_ids + p.slots + S + 64) * Hkv * 4;
-    if (blocks > INT32_MAX || p.slots > 65535) return fail(RPA_ERR_UNSUPPORTED, "%s: T=%d tokens of %d heads are too many workgroups", who, T, Hkv);
+    // a launch holds less than 2^32 threads, 512 a workgroup
+    const int64_t blocks = ((int64_t)p.first_ids + p.slots + S) * Hkv * ((Dv + 127) / 128) + 64;
+    if (blocks >= (int64_t)1 << 23 || p.slots > 65535)
+      return fail(RPA_ERR_UNSUPPORTED, "%s: T=%d tokens in %d sequences of %d heads are too many workgroups", who, T, S, Hkv);
     return hip_fail(rpa::launch_decay_chunk(s, p), "rpa_decay_linear_attention chunk launch");
   }
   return hip_fail(rpa::launch_decay_recurrent(s, p), "rpa_decay_linear_attention launch");

@@ -381,7 +381,8 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
  * A slot outside [0, num_slots) reads as a zero state and is not written.  Sequences without tokens keep their slots as they are
  * (nothing is copied to state_out_indices either).  State and sums are float32 throughout.
  * A value that is not finite reaches its own and later tokens of its sequence only.
- * Limits: Dk, Dv multiples of 4, at most 256; Hq a multiple of Hkv; S at most 65000.
+ * Limits: Dk, Dv multiples of 4, at most 256; Hq a multiple of Hkv; S at most 65000, and (2 S + T / 64) * Hkv * ceil(Dv / 128) below
+ * 2^23 (workgroups of a launch).
  */
 int rpa_decay_linear_attention(rpa_stream_t stream, const void* query, const void* key, const void* value, const float* log_decay,
                                float* state, const int32_t* state_indices, const int32_t* state_out_indices,

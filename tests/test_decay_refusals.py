@@ -28,6 +28,13 @@ def test_the_c_entry_refuses(over, text, code):
     assert text in lib.rpa_last_error().decode()
 
 
+def test_more_workgroups_than_a_launch_holds_are_refused():
+    lib = _lib.load()
+    big = dict(T=10_000_000, S=65_000, Hq=1000, Hkv=1000, Dk=4, Dv=4, qs=4000, ks=4000, vs=4000)
+    assert _call(lib, **big) == -2
+    assert "too many workgroups" in lib.rpa_last_error().decode()
+
+
 def test_an_empty_batch_is_a_no_op():
     assert _call(_lib.load(), T=0) == 0
 
