@@ -11,6 +11,7 @@
 // launched where the bounds allow a sequence of more than one segment.  The first segments are numbered by sequence or by
 // floor(qsl[i] / (kDecayRows + 1)), the others by floor(qsl[i] / seg_len) + j - 1: both are distinct without a plan, since such
 // a sequence is longer than the divisor.
+#include "rpa_decay_factor.h"
 #include "rpa_decay_steps.h"
 #include "rpa_mfma.h"
 
@@ -380,12 +381,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_k
 #pragma unroll
   for (int d = 0; d < ND; ++d) S[d] = f32x4{};
   if constexpr (OUT) load_state<ND, true>(p, g, h, c0 / 16 + w, lane, S);
-  // The state is multiplied by l^C = full.x + full.y once a chunk: each factor is rounded so that the product of all of them so
-  // far stays within a rounding of the true power (`off`: how far it is, relatively), however long the segment.
   const float rate = p.log_decay[h];
   const float2 full = decay_power(rate, kChunk);
-  const float per = full.x > 0.f ? 1.f / full.x : 0.f;
-  float off = 0.f;
+  DecayFactor factor;
+  factor.init(full.x, full.y);
   double over = 1.0;
   if (tid <= kChunk) pw[tid] = decay_float(rate, tid);
   if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_float(rate, kChunk - 1 - (tid - 64));
@@ -502,8 +501,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 128 ? 4 : 2) void decay_chunk_bf16_k
     // their tokens enter with their decay to the end of the segment, which leaves the state alone.
     float behind = 1.f;
     if constexpr (OUT) {
-      float l = n < kChunk ? pw[n] : full.x + (full.y - full.x * off);
-      off += ((l - full.x) - full.y) * per;
+      const float l = n < kChunk ? pw[n] : factor.next();
 #pragma unroll
       for (int d = 0; d < ND; ++d) S[d] *= l;
     } else {
@@ -622,8 +620,8 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
   if constexpr (OUT) load_state<ND, false>(p, g, h, c0 / 16 + w, lane, S);
   const float rate = p.log_decay[h];
   const float2 full = decay_power(rate, kChunk);
-  const float per = full.x > 0.f ? 1.f / full.x : 0.f;
-  float off = 0.f;
+  DecayFactor factor;
+  factor.init(full.x, full.y);
   double over = 1.0;
   if (tid <= kChunk) pw[tid] = decay_float(rate, tid);
   if (tid >= 64 && tid < 64 + kChunk) left[tid - 64] = decay_float(rate, kChunk - 1 - (tid - 64));
@@ -729,8 +727,7 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_wide_kernel(DecayParams p
     if (OUT && c == chunks - 1 && (!g.last || g.out < 0)) break;  // nobody reads the state behind this chunk
     float behind = 1.f;
     if constexpr (OUT) {
-      const float l = n < kChunk ? pw[n] : full.x + (full.y - full.x * off);
-      off += ((l - full.x) - full.y) * per;
+      const float l = n < kChunk ? pw[n] : factor.next();
 #pragma unroll
       for (int d = 0; d < ND; ++d) S[d] *= l;
     } else {
