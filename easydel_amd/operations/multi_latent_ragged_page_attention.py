@@ -7,6 +7,9 @@ Where the reference hands the arrays to ``ejkernel.modules.multi_latent_ragged_p
 v2 :1019-1030, :1090-1101) this module hands device pointers to ``librpa_hip.so``.  The two versions differ in the
 reference only by the block-size hints they pass to ejkernel; here they are one implementation.  The shard-local path
 over the ``ATTN_DP`` mesh axis (:437-560) has no one-GPU counterpart.
+
+``rope=`` (an ``operations.Rotary``), an addition to the reference's signature, hands the operation ``queries_pe`` and ``keys_pe``
+that are not rotated yet, in any layout and type that the call without it takes.
 """
 
 from __future__ import annotations
@@ -20,6 +23,7 @@ from ..caching.mla_ragged_page import MLARaggedPagesCacheView
 from ._attention_outputs import AttentionOutput
 from ._base_operation import OperationImpl, OperationRegistry
 from .requirements import CacheType, ExecutionMode, MetadataField, OperationRequirements, RequirementsBuilder
+from .rotary import rotation_operands
 
 logger = logging.getLogger(__name__)
 
@@ -119,12 +123,13 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
         if rope is not None:
             # unrotated queries_pe and keys_pe: one launch rotates both and writes the latent rows, then the attention reads
             distribution = _resolve_distribution(cache_metadata)
+            queries_pe, keys_pe = rotation_operands(queries_nope.dtype, queries_pe, keys_pe)
             queries_pe, _ = kernels.rope_mla_page_scatter(
-                queries_pe, keys_values.to(kv_pages.dtype).contiguous(), keys_pe, kv_pages,  # (both of one type: rounding ahead of the rotation is the caller's)
+                queries_pe, keys_values.to(kv_pages.dtype).contiguous(), keys_pe, kv_pages,
                 rope.cos_sin, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc,
                 distribution[2:3], positions=rope_positions, is_neox_style=rope.is_neox_style)
             output, _ = kernels.mla_ragged_paged_attention(
-                queries_nope.contiguous(), queries_pe, None, None, kv_pages, cache_metadata.context_lens,
+                queries_nope.contiguous(), queries_pe.to(queries_nope.dtype), None, None, kv_pages, cache_metadata.context_lens,
                 cache_metadata.pages_tables.reshape(-1), cache_metadata.query_start_loc,
                 torch.stack([torch.zeros_like(distribution[2]), torch.zeros_like(distribution[2]), distribution[2]]),
                 softmax_scale=softmax_scale, sliding_window=sliding_window, logits_soft_cap=logits_soft_cap, softmax_aux=softmax_aux)

@@ -31,3 +31,19 @@ class Rotary:
         inv = theta ** (-torch.arange(0, rope_dim, 2, dtype=torch.float64) / rope_dim)
         angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * inv
         return cls(torch.cat((angle.cos(), angle.sin()), dim=1).to(torch.float32).to(device), is_neox_style)
+
+
+def token_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [T, ...]`` with token rows that a kernel reads in place: contiguous each, however far apart.  Rows of a projection are; parts of
+    every head (and one row for all tokens) are copied."""
+    if t.is_contiguous() or t.shape[0] == 0:
+        return t
+    return t if t[0].is_contiguous() and (t.shape[0] == 1 or t.stride(0) >= t[0].numel()) else t.contiguous()
+
+
+def rotation_operands(result: torch.dtype, *operands: torch.Tensor) -> list[torch.Tensor]:
+    """The operands as the rotating writes read them: of one type, token rows in place.  Where types differ, among them or from that of
+    the ``result``, they meet in float32, which holds 16-bit values as they are: what is rounded is the result, once."""
+    if any(t.dtype != result for t in operands):
+        operands = [t.to(torch.float32) for t in operands]
+    return [token_rows(t) for t in operands]

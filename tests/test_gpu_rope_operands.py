@@ -1,0 +1,47 @@
+"""GPU tests of the operations with ``rope=`` on the operands that layers have in hand: parts of their projections, types that differ."""
+
+import numpy as np
+import pytest
+import torch
+
+from easydel_amd.caching import MLARaggedPagesCacheConfig, MLARaggedPagesCacheView, RaggedPagesMetadata
+from easydel_amd.operations import OperationMetadata, OperationRegistry, Rotary
+from rope_testlib import BF16, F32, decode, encode, rotate, tl
+from test_gpu_hybrid_step import _steps
+
+pytestmark = pytest.mark.gpu
+
+TYPE = {BF16: torch.bfloat16, F32: torch.float32}
+
+
+def _draw(rng, gpu, tag, *shape):
+    raw = encode(rng.standard_normal(shape).astype(np.float32), tag)
+    return decode(raw, tag), tl.to_torch(raw, tag, gpu)
+
+
+def _turned(x, pos, tab, neox, gpu):
+    """Rotated in float32, rounded once to bfloat16."""
+    rows = tab[np.clip(pos, 0, len(tab) - 1)]
+    return tl.to_torch(encode(rotate(x, rows, tab.shape[1], neox), BF16), BF16, gpu)
+
+
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("q_tag,k_tag", [(BF16, BF16), (F32, BF16), (BF16, F32), (F32, F32)])
+def test_multi_latent_operation_with_rope_on_parts_of_projections(gpu, q_tag, k_tag, neox):
+    """Queries are the tail of every head of one projection, latent rows and rope keys the two ends of another's rows."""
+    rng = np.random.default_rng(17)
+    H, rank, nope, R = 16, 512, 128, 64
+    config = MLARaggedPagesCacheConfig.create(torch.bfloat16, 1, 1, 256, kv_lora_rank=rank, qk_rope_head_dim=R, page_size=32, num_pages=41)
+    a, b = (MLARaggedPagesCacheView.init(config, device=gpu) for _ in range(2))
+    op = OperationRegistry.create("multi_latent_ragged_page_attention_v2", OperationMetadata())
+    rope = Rotary.create(R, 256, is_neox_style=neox, device=gpu)
+    tab = rope.cos_sin.cpu().numpy()
+    for fields, T, pos in _steps(32):
+        meta = RaggedPagesMetadata.from_numpy(fields, version="v3", page_size=32, device=gpu)
+        (_, absorbed), (q32, q), (kv32, kv) = _draw(rng, gpu, BF16, T, H, rank), _draw(rng, gpu, q_tag, T, H, nope + R), _draw(rng, gpu, k_tag, T, rank + R)
+        latent, pe = kv.split([rank, R], -1)
+        got = op(absorbed, q[..., nope:], latent, pe, a, meta, softmax_scale=192 ** -0.5, rope=rope).attention_outputs
+        want = op(absorbed, _turned(q32[..., nope:], pos, tab, neox, gpu), latent, _turned(kv32[:, None, rank:], pos, tab, neox, gpu)[:, 0], b, meta,
+                  softmax_scale=192 ** -0.5).attention_outputs
+        torch.cuda.synchronize()
+        assert got.dtype == torch.bfloat16 and torch.equal(a.kv_pages, b.kv_pages) and torch.equal(got, want)

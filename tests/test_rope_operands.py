@@ -1,0 +1,70 @@
+"""CPU tests of what the operations hand to the rotating writes: the operands of the call without ``rope=`` are taken with it too."""
+
+import pytest
+import torch
+
+from easydel_amd import kernels
+from easydel_amd.caching import (MLARaggedPagesCacheConfig, MLARaggedPagesCacheView,
+                                 RaggedPagesMetadata)
+from easydel_amd.operations import OperationMetadata, OperationRegistry, Rotary
+
+T = 5
+
+
+def _meta():
+    return RaggedPagesMetadata.create_empty(T, 2, 2, page_size=16, version="v3", device="cpu")
+
+
+def _rows_in_place(t):
+    return t[0].is_contiguous() and t.stride(0) >= t[0].numel()
+
+
+@pytest.fixture
+def latent(monkeypatch):
+    """The multi-latent operation with its two kernel calls recorded."""
+    seen = {}
+
+    def write(queries_pe, keys_values, keys_pe, kv_pages, *a, **k):
+        seen["write"] = (queries_pe, keys_values, keys_pe)
+        return torch.empty_like(queries_pe).contiguous(), kv_pages
+
+    def read(queries_nope, queries_pe, *a, **k):
+        seen["read"] = (queries_nope, queries_pe)
+        return torch.empty_like(queries_nope), None
+
+    monkeypatch.setattr(kernels, "rope_mla_page_scatter", write)
+    monkeypatch.setattr(kernels, "mla_ragged_paged_attention", read)
+    op = OperationRegistry.create("multi_latent_ragged_page_attention_v2", OperationMetadata())
+    config = MLARaggedPagesCacheConfig.create(torch.bfloat16, 1, 1, 64, kv_lora_rank=128, qk_rope_head_dim=64, page_size=16, num_pages=3)
+    view = MLARaggedPagesCacheView.init(config, device="cpu")
+    rope = Rotary.create(64, 64, device="cpu")
+
+    def run(nope, pe, kv, kpe):
+        op(nope, pe, kv, kpe, view, _meta(), rope=rope)
+        return seen
+
+    return run
+
+
+def _latent_operands(dtype=torch.bfloat16):
+    q = torch.zeros(T, 3, 96 + 64, dtype=dtype)  # heads of one projection: the part without a position, then the rope part
+    kv = torch.zeros(T, 128 + 64, dtype=dtype)
+    return torch.zeros(T, 3, 128, dtype=dtype), q.split([96, 64], -1)[1], *kv.split([128, 64], -1)
+
+
+def test_multi_latent_takes_the_parts_of_its_projections(latent):
+    nope, pe, kv, kpe = _latent_operands()
+    assert not pe[0].is_contiguous()
+    seen = latent(nope, pe, kv, kpe)
+    assert all(_rows_in_place(t) for t in seen["write"]) and seen["write"][1].is_contiguous()
+    assert seen["write"][2].data_ptr() == kpe.data_ptr()  # whole rows stay where they are
+
+
+@pytest.mark.parametrize("pe_type,kpe_type", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32),
+                                              (torch.float16, torch.float16)])
+def test_multi_latent_takes_types_that_differ(latent, pe_type, kpe_type):
+    """Rotated in float32, and only the result in the type of ``queries_nope``."""
+    nope, pe, kv, kpe = _latent_operands()
+    seen = latent(nope, pe.to(pe_type), kv, kpe.to(kpe_type))
+    assert seen["write"][0].dtype == seen["write"][2].dtype == torch.float32
+    assert seen["read"][1].dtype == torch.bfloat16
