@@ -9,8 +9,8 @@ the cache dtype with a warning when it narrows (:570-580), write-back of the upd
 :732-746), this module hands device pointers to ``librpa_hip.so`` through ``easydel_amd.kernels``.
 
 ``rope=`` (an ``operations.Rotary``), an addition to the reference's signature, hands the v3 operation queries and keys that
-are not rotated yet: the page write rotates them on the way (``rope_positions [T]`` where the angles go by something else than
-the cache positions).
+are not rotated yet, in any layout and type that the call without it takes: the page write rotates them on the way
+(``rope_positions [T]`` where the angles go by something else than the cache positions).
 """
 
 from __future__ import annotations
@@ -24,6 +24,7 @@ from ..caching.ragged_page import RaggedPagesCacheView, RaggedPagesMetadata
 from ._attention_outputs import AttentionOutput
 from ._base_operation import OperationImpl, OperationRegistry
 from .requirements import CacheType, ExecutionMode, MetadataField, OperationRequirements, RequirementsBuilder
+from .rotary import rotation_operands
 
 logger = logging.getLogger(__name__)
 
@@ -93,9 +94,11 @@ class _RaggedPageAttn(OperationImpl):
             # the attention reads
             if key is None or value is None:
                 raise ValueError("ragged_page_attention_v3 with `rope` needs the step's key and value")
+            dtype = query.dtype
+            query, key, value = rotation_operands(dtype, query, key, value)
             query = cache_view.rope_concatenate_to_cache(query, key, value, cache_metadata, rope, positions=rope_positions)
             output = kernels.ragged_paged_attention(
-                query, kv_pages, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1),
+                query.to(dtype), kv_pages, cache_metadata.context_lens, cache_metadata.pages_tables.reshape(-1),
                 cache_metadata.query_start_loc, cache_metadata.request_distribution[2:3], softmax_scale=softmax_scale,
                 sliding_window=sliding_window, logits_soft_cap=logits_soft_cap, kv_scales=getattr(cache_view, "kv_scales", None),
                 num_kv_heads=key.shape[1], softmax_aux=softmax_aux)

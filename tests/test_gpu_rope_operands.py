@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from easydel_amd.caching import MLARaggedPagesCacheConfig, MLARaggedPagesCacheView, RaggedPagesMetadata
+from easydel_amd.caching import (MLARaggedPagesCacheConfig, MLARaggedPagesCacheView, RaggedPagesCacheConfig, RaggedPagesCacheView,
+                                 RaggedPagesMetadata)
 from easydel_amd.operations import OperationMetadata, OperationRegistry, Rotary
 from rope_testlib import BF16, F32, decode, encode, rotate, tl
 from test_gpu_hybrid_step import _steps
@@ -45,3 +46,25 @@ def test_multi_latent_operation_with_rope_on_parts_of_projections(gpu, q_tag, k_
                   softmax_scale=192 ** -0.5).attention_outputs
         torch.cuda.synchronize()
         assert got.dtype == torch.bfloat16 and torch.equal(a.kv_pages, b.kv_pages) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("q_tag,kv_tag", [(BF16, BF16), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize("kvdtype", [torch.bfloat16, torch.float32])
+def test_v3_operation_with_rope_on_parts_of_heads_and_other_types(gpu, kvdtype, q_tag, kv_tag):
+    """Heads of 64 that are the front of heads of 80 of one projection."""
+    rng = np.random.default_rng(18)
+    Hq, Hkv, D = 4, 2, 64
+    config = RaggedPagesCacheConfig.create(kvdtype, 1, Hkv, 256, kv_head_dim_size=D, page_size=32, num_pages=41)
+    a, b = (RaggedPagesCacheView.init(config, device=gpu) for _ in range(2))
+    op = OperationRegistry.create("ragged_page_attention_v3", OperationMetadata())
+    rope = Rotary.create(D, 256, device=gpu)
+    tab = rope.cos_sin.cpu().numpy()
+    for fields, T, pos in _steps(32):
+        meta = RaggedPagesMetadata.from_numpy(fields, version="v3", page_size=32, device=gpu)
+        (q32, q), (k32, k), (_, v) = _draw(rng, gpu, q_tag, T, Hq, 80), _draw(rng, gpu, kv_tag, T, Hkv, 80), _draw(rng, gpu, kv_tag, T, Hkv, 80)
+        got = op(q[..., :D], k[..., :D], v[..., :D], a, meta, rope=rope).attention_outputs
+        rows = tab[np.clip(pos, 0, len(tab) - 1)]
+        turned = lambda x: torch.from_numpy(rotate(x[..., :D], rows, D, True)).to(gpu)  # noqa: E731
+        want = op(turned(q32).to(TYPE[q_tag]), turned(k32), v[..., :D], b, meta).attention_outputs
+        torch.cuda.synchronize()
+        assert got.dtype == TYPE[q_tag] and torch.equal(a.kv_pages, b.kv_pages) and torch.equal(got, want)

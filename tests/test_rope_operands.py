@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from easydel_amd import kernels
-from easydel_amd.caching import (MLARaggedPagesCacheConfig, MLARaggedPagesCacheView,
+from easydel_amd.caching import (MLARaggedPagesCacheConfig, MLARaggedPagesCacheView, RaggedPagesCacheConfig, RaggedPagesCacheView,
                                  RaggedPagesMetadata)
 from easydel_amd.operations import OperationMetadata, OperationRegistry, Rotary
 
@@ -68,3 +68,49 @@ def test_multi_latent_takes_types_that_differ(latent, pe_type, kpe_type):
     seen = latent(nope, pe.to(pe_type), kv, kpe.to(kpe_type))
     assert seen["write"][0].dtype == seen["write"][2].dtype == torch.float32
     assert seen["read"][1].dtype == torch.bfloat16
+
+
+@pytest.fixture
+def v3(monkeypatch):
+    """The v3 operation with its two kernel calls recorded."""
+    seen = {}
+
+    def write(query, key, value, kv_pages, *a, kv_scales=None, **k):
+        seen["write"] = (query, key, value)
+        out = torch.empty_like(query).contiguous()
+        return (out, kv_pages) if kv_scales is None else (out, kv_pages, kv_scales)
+
+    def read(query, *a, **k):
+        seen["read"] = query
+        return torch.empty_like(query)
+
+    monkeypatch.setattr(kernels, "rope_page_scatter_ragged", write)
+    monkeypatch.setattr(kernels, "ragged_paged_attention", read)
+    op = OperationRegistry.create("ragged_page_attention_v3", OperationMetadata())
+    rope = Rotary.create(64, 64, device="cpu")
+
+    def run(q, k, v, kvdtype=torch.bfloat16, scaled=None):
+        config = RaggedPagesCacheConfig.create(kvdtype, 1, 2, 64, kv_head_dim_size=64, page_size=16, num_pages=3)
+        op(q, k, v, RaggedPagesCacheView.init(config, device="cpu", scaled=scaled), _meta(), rope=rope)
+        return seen
+
+    return run
+
+
+def test_v3_takes_parts_of_every_head(v3):
+    q, k, v = (torch.zeros(T, h, 80, dtype=torch.bfloat16)[..., :64] for h in (4, 2, 2))
+    seen = v3(q, k, v)
+    assert all(_rows_in_place(t) for t in seen["write"])
+    assert all(_rows_in_place(t) for t in v3(*(torch.zeros(1, h, 64).expand(T, h, 64) for h in (4, 2, 2)))["write"])  # one row for all tokens
+    qkv = torch.zeros(T, 8 * 64, dtype=torch.bfloat16)
+    views = [x.unflatten(1, (-1, 64)) for x in qkv.split((256, 128, 128), 1)]
+    seen = v3(*views)
+    assert [t.data_ptr() for t in seen["write"]] == [t.data_ptr() for t in views]  # rows of a projection are read in place
+
+
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.float32, torch.float32), (torch.float32, torch.bfloat16, torch.bfloat16),
+                                   (torch.bfloat16, torch.bfloat16, torch.float32), (torch.bfloat16, torch.float16, torch.float16)])
+def test_v3_takes_types_that_differ(v3, types):
+    seen = v3(*(torch.zeros(T, h, 64, dtype=t) for h, t in zip((4, 2, 2), types)))
+    assert {t.dtype for t in seen["write"]} == {torch.float32}
+    assert seen["read"].dtype == types[0]
