@@ -120,6 +120,9 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
             raise ValueError("`keys_pe` token dimension must match `queries_nope` token dimension. "
                              f"Got keys_pe={keys_pe.shape[0]} vs queries_nope={queries_nope.shape[0]}.")
         kv_pages = cache_view.kv_pages
+        if kv_pages.element_size() < max(keys_values.element_size(), keys_pe.element_size()):
+            logger.warning("Casting keys_values/keys_pe from %s to lower-precision KV cache dtype %s; "
+                           "this may reduce numerical fidelity.", keys_values.dtype, kv_pages.dtype)
         if rope is not None:
             # unrotated queries_pe and keys_pe: one launch rotates both and writes the latent rows, then the attention reads
             distribution = _resolve_distribution(cache_metadata)
@@ -135,9 +138,6 @@ class _MultiLatentRaggedPageAttn(OperationImpl):
                 softmax_scale=softmax_scale, sliding_window=sliding_window, logits_soft_cap=logits_soft_cap, softmax_aux=softmax_aux)
             return AttentionOutput(attention_weights=None, attention_outputs=output.reshape(shape4) if is_4d else output, cache_view=cache_view)
         if keys_values.dtype != kv_pages.dtype or keys_pe.dtype != kv_pages.dtype:
-            if kv_pages.element_size() < max(keys_values.element_size(), keys_pe.element_size()):
-                logger.warning("Casting keys_values/keys_pe from %s to lower-precision KV cache dtype %s; "
-                               "this may reduce numerical fidelity.", keys_values.dtype, kv_pages.dtype)
             keys_values = keys_values.to(kv_pages.dtype)
             keys_pe = keys_pe.to(kv_pages.dtype)
         distribution = _resolve_distribution(cache_metadata)

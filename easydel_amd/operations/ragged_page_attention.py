@@ -94,6 +94,8 @@ class _RaggedPageAttn(OperationImpl):
             # the attention reads
             if key is None or value is None:
                 raise ValueError("ragged_page_attention_v3 with `rope` needs the step's key and value")
+            if getattr(cache_view, "kv_scales", None) is None:
+                _warn_of_narrowing(key, value, kv_pages)
             dtype = query.dtype
             query, key, value = rotation_operands(dtype, query, key, value)
             query = cache_view.rope_concatenate_to_cache(query, key, value, cache_metadata, rope, positions=rope_positions)
@@ -123,9 +125,7 @@ class _RaggedPageAttn(OperationImpl):
             cache_view.kv_pages, cache_view.kv_scales = kv_pages, kv_scales
             return AttentionOutput(attention_weights=None, attention_outputs=output, cache_view=cache_view)
         if key.dtype != kv_pages.dtype or value.dtype != kv_pages.dtype:
-            if kv_pages.element_size() < max(key.element_size(), value.element_size()):
-                logger.warning("Casting key/value from %s to lower-precision KV cache dtype %s; "
-                               "this may reduce numerical fidelity.", key.dtype, kv_pages.dtype)
+            _warn_of_narrowing(key, value, kv_pages)
             key = key.to(kv_pages.dtype)
             value = value.to(kv_pages.dtype)
         output, kv_pages = kernels.ragged_paged_attention_v3(
@@ -218,6 +218,12 @@ def dp_local_reduce(local_outputs) -> torch.Tensor:
     for other in local_outputs[1:]:
         total = total + other.to(torch.float32)
     return total.to(local_outputs[0].dtype)
+
+
+def _warn_of_narrowing(key, value, kv_pages) -> None:
+    if kv_pages.element_size() < max(key.element_size(), value.element_size()):
+        logger.warning("Casting key/value from %s to lower-precision KV cache dtype %s; "
+                       "this may reduce numerical fidelity.", key.dtype, kv_pages.dtype)
 
 
 def _num_kv_heads(cache_view) -> int | None:

@@ -114,3 +114,19 @@ def test_v3_takes_types_that_differ(v3, types):
     seen = v3(*(torch.zeros(T, h, 64, dtype=t) for h, t in zip((4, 2, 2), types)))
     assert {t.dtype for t in seen["write"]} == {torch.float32}
     assert seen["read"].dtype == types[0]
+
+
+def test_narrowing_is_told_with_rope_as_without(latent, v3, caplog):
+    """Rows of a wider type than the pages are cast with a warning; scaled pages are coded, which is no cast."""
+    wide, narrow = torch.float32, torch.bfloat16
+    ops = _latent_operands()
+    for kv, kpe, told in ((narrow, narrow, False), (wide, narrow, True), (narrow, wide, True)):
+        caplog.clear()
+        latent(*ops[:2], ops[2].to(kv), ops[3].to(kpe))
+        assert ("lower-precision KV cache dtype" in caplog.text) == told
+    q, k = torch.zeros(T, 4, 64, dtype=narrow), torch.zeros(T, 2, 64, dtype=narrow)
+    for key, value, kvdtype, scaled, told in ((k, k, narrow, None, False), (k.to(wide), k, narrow, None, True), (k, k.to(wide), narrow, None, True),
+                                              (k, k, torch.float8_e4m3fn, None, True), (k, k, torch.float8_e4m3fn, True, False), (k, k, torch.int8, None, False)):
+        caplog.clear()
+        v3(q, key, value, kvdtype, scaled)
+        assert ("lower-precision KV cache dtype" in caplog.text) == told
