@@ -482,12 +482,16 @@ def _on(t: torch.Tensor, name: str, dtype: torch.dtype, device) -> int:
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
+    if t.is_contiguous():
+        start = t.data_ptr()
+        return start, start + t.nbytes
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
 def _turned_out(query, query_out, others, name: str):
-    """The tensor the turned queries go to: a new one, the queries themselves, or one that overlaps no operand."""
+    """The tensor the turned queries go to: a new one, the queries themselves, or one that overlaps no operand (``others``: all of them but
+    the queries; None: not given)."""
     if query_out is None:
         return torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
     if query_out.shape != query.shape or query_out.dtype != query.dtype or query_out.device != query.device:
@@ -498,6 +502,8 @@ def _turned_out(query, query_out, others, name: str):
     a, b = _span(query_out)
     in_place = query_out.data_ptr() == query.data_ptr() and query.is_contiguous()
     for t in others if in_place else (query, *others):
+        if t is None:
+            continue
         c, d = _span(t)
         if a < d and c < b:
             raise ValueError(f"{name} overlaps another operand (only the contiguous queries themselves may be given)")
@@ -566,7 +572,7 @@ def rope_page_scatter_ragged(query, key, value, kv_pages, cos_sin, context_lens,
     dev = query.device
     table, rope, rows = _table(cos_sin, None, D, dev)
     S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
-    out = _turned_out(query, query_out, (key, value), "query_out")
+    out = _turned_out(query, query_out, (key, value, kv_pages, kv_scales, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs), "query_out")
     pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
     scales = None if kv_scales is None else _on(kv_scales, "kv_scales", torch.float32, dev)
     if T > 0:
@@ -590,7 +596,7 @@ def rope_unified_page_scatter(query, key, value, key_cache, value_cache, cos_sin
     kd, dev = dtype_tag(key_cache.dtype), query.device
     table, rope, rows = _table(cos_sin, None, D, dev)
     S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
-    out = _turned_out(query, query_out, (key, value), "query_out")
+    out = _turned_out(query, query_out, (key, value, key_cache, value_cache, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs), "query_out")
     kc, vc = _on(key_cache, "key_cache", key_cache.dtype, dev), _on(value_cache, "value_cache", key_cache.dtype, dev)
     if T > 0:
         _launch(dev, lib.rpa_rope_unified_page_scatter, q, k, v, out.data_ptr(), kc, vc, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, Hkv, D, rope, rows,
@@ -622,7 +628,8 @@ def rope_mla_page_scatter(queries_pe, keys_values, keys_pe, kv_pages, cos_sin, c
     latent = _on(keys_values, "keys_values", kv_pages.dtype, dev)
     table, _, rows = _table(cos_sin, rope, rope, dev)
     S, M, ctx, bt, qsl, ns, pos = _ragged(context_lens, block_tables, query_start_loc, num_seqs, positions, T, dev)
-    out = _turned_out(queries_pe, query_out, (keys_pe, keys_values), "query_out")
+    out = _turned_out(queries_pe, query_out, (keys_pe, keys_values, kv_pages, cos_sin, positions, context_lens, block_tables, query_start_loc, num_seqs),
+                      "query_out")
     pages = _on(kv_pages, "kv_pages", kv_pages.dtype, dev)
     if T > 0:
         _launch(dev, lib.rpa_rope_mla_page_scatter, q, latent, k, out.data_ptr(), pages, table, pos, ctx, bt, qsl, ns, T, S, M, P, pg, Hq, lkv, rope, row, rows,

@@ -100,3 +100,47 @@ def test_the_rotation_oracle_turns_by_the_angle():
         pair = (lambda a: a[..., :4] + 1j * a[..., 4:]) if neox else (lambda a: a[..., 0::2] + 1j * a[..., 1::2])
         angle = np.arange(50)[:, None, None] * 10000.0 ** (-np.arange(0, 8, 2) / 8)
         assert np.abs(pair(y) - pair(x) * np.exp(1j * angle)).max() < 1e-6
+
+
+def _unchecked(monkeypatch):
+    """The wrappers on CPU tensors: everything but where memory lies."""
+    def rows(t, name, shape, dtype, device):
+        return t.data_ptr(), t.stride(0)
+
+    monkeypatch.setattr(kernels, "_rows", rows)
+    monkeypatch.setattr(kernels, "_on", lambda t, *a: t.data_ptr())
+    monkeypatch.setattr(kernels, "_launch", lambda *a: None)
+
+
+I = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+
+
+@pytest.mark.parametrize("what", ["pages", "scales", "table", "positions", "context_lens", "pool", "latent"])
+def test_turned_queries_may_not_go_into_any_operand(monkeypatch, what):
+    """``query_out`` inside the pages, the scales, the table or the metadata."""
+    _unchecked(monkeypatch)
+    q, k = torch.zeros(2, 2, 64), torch.zeros(2, 1, 64)
+    inside = torch.zeros(4096)
+    out = inside[256:512].view(2, 2, 64)
+    pages, table = torch.zeros(2, 4, 2, 64), torch.zeros(10, 64)
+    meta = dict(context_lens=I(2), block_tables=I(0), query_start_loc=I(0, 2), num_seqs=I(1))
+    with pytest.raises(ValueError, match="query_out overlaps another operand"):
+        if what == "pages":
+            kernels.rope_page_scatter_ragged(q, k, k, inside[:1024].view(2, 4, 2, 64), table, **meta, query_out=out)
+        elif what == "scales":
+            kernels.rope_page_scatter_ragged(q, k, k, torch.zeros(256, 4, 2, 64, dtype=torch.int8), table, **meta, kv_scales=inside[:512], query_out=out)
+        elif what == "table":
+            kernels.rope_page_scatter_ragged(q, k, k, pages, inside[:640].view(10, 64), **meta, query_out=out)
+        elif what == "positions":
+            kernels.rope_page_scatter_ragged(q, k, k, pages, table, **meta, positions=inside.view(torch.int32)[300:302], query_out=out)
+        elif what == "context_lens":
+            kernels.rope_page_scatter_ragged(q, k, k, pages, table, **{**meta, "context_lens": inside.view(torch.int32)[511:512]}, query_out=out)
+        elif what == "pool":
+            kernels.rope_unified_page_scatter(q, k, k, torch.zeros(4, 4, 1, 64), inside[:1024].view(4, 4, 1, 64), table, **meta, query_out=out)
+        else:
+            kernels.rope_mla_page_scatter(q, torch.zeros(2, 128), k[:, 0], inside[:1024].view(1, 4, 256), table, **meta, query_out=out)
+    for fine in (None, q, inside[1024:1280].view(2, 2, 64)):  # beside them is fine
+        got, _ = kernels.rope_page_scatter_ragged(q, k, k, inside[:1024].view(2, 4, 2, 64), table, **meta, query_out=fine)
+        assert fine is None or got is fine
+    with pytest.raises(ValueError, match="overlaps another operand"):  # in place, too
+        kernels.rope_page_scatter_ragged(out, k, k, inside[:1024].view(2, 4, 2, 64), table, **meta, query_out=out)
