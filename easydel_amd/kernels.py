@@ -682,7 +682,11 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
         raise ValueError(f"out must be [{T}, {Hq}, {Dv}], got {list(out.shape)}")
     else:
         a, b = _span(out)
-        for name, t in (("query", query), ("key", key), ("value", value), ("state", state)):
+        for name, t in (("query", query), ("key", key), ("value", value), ("state", state), ("log_decay", log_decay), ("state_indices", state_indices),
+                        ("state_out_indices", state_out_indices), ("context_lens", context_lens), ("query_start_loc", query_start_loc),
+                        ("num_seqs", num_seqs)):
+            if t is None:
+                continue
             c, d = _span(t)
             if a < d and c < b:
                 raise ValueError(f"out overlaps {name}")

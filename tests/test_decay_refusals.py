@@ -49,3 +49,20 @@ def test_the_wrapper_refuses():
         call(q=q[0])
     with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
         call(q=q.double())
+
+
+@pytest.mark.parametrize("what", ["log_decay", "state_indices", "state_out_indices", "context_lens", "query_start_loc", "num_seqs"])
+def test_the_output_may_not_lie_in_any_operand(monkeypatch, what):
+    monkeypatch.setattr(kernels, "_rows", lambda t, *a: (t.data_ptr(), t.stride(0)))  # CPU tensors: everything but where memory lies
+    monkeypatch.setattr(kernels, "_on", lambda t, *a: t.data_ptr())
+    monkeypatch.setattr(kernels, "_launch", lambda *a: None)
+    I = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    q, inside = torch.zeros(2, 1, 64), torch.zeros(512)
+    given = dict(log_decay=torch.zeros(1), state=torch.zeros(3, 1, 64, 64), state_indices=I(0), query_start_loc=I(0, 2), num_seqs=I(1), context_lens=I(2),
+                 state_out_indices=I(1))
+    out = inside[128:256].view(2, 1, 64)
+    got, _ = kernels.decay_linear_attention(q, q, q, **given, out=out)
+    assert got is out
+    given[what] = inside[254:254 + given[what].numel()].view(given[what].dtype)
+    with pytest.raises(ValueError, match=f"out overlaps {what}"):
+        kernels.decay_linear_attention(q, q, q, **given, out=out)
