@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from easydel_amd.caching import (MLARaggedPagesCacheConfig, MLARaggedPagesCacheView, RaggedPagesCacheConfig, RaggedPagesCacheView,
-                                 RaggedPagesMetadata)
+from easydel_amd.caching import (DecayStateCacheConfig, DecayStateCacheView, DecayStateMetadata, MLARaggedPagesCacheConfig, MLARaggedPagesCacheView,
+                                 RaggedPagesCacheConfig, RaggedPagesCacheView, RaggedPagesMetadata)
 from easydel_amd.operations import OperationMetadata, OperationRegistry, Rotary
 from rope_testlib import BF16, F32, decode, encode, rotate, tl
 from test_gpu_hybrid_step import _steps
@@ -68,3 +68,20 @@ def test_v3_operation_with_rope_on_parts_of_heads_and_other_types(gpu, kvdtype, 
         want = op(turned(q32).to(TYPE[q_tag]), turned(k32), v[..., :D], b, meta).attention_outputs
         torch.cuda.synchronize()
         assert got.dtype == TYPE[q_tag] and torch.equal(a.kv_pages, b.kv_pages) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tag", [BF16, F32])
+def test_linear_layer_on_parts_of_heads(gpu, tag):
+    rng = np.random.default_rng(19)
+    T, H, D = 70, 3, 64
+    _, heads = _draw(rng, gpu, tag, T, H, 3 * D)
+    parts = heads.split(D, -1)
+    one = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    meta = DecayStateMetadata(query_start_loc=one(0, 69, 70), num_seqs=one(2), state_indices=one(2, 0))
+    decays = torch.tensor([-0.1, -1.0, -3.0], device=gpu)
+    op = OperationRegistry.create("ragged_decay_linear_attention", OperationMetadata())
+    views = [DecayStateCacheView.init(DecayStateCacheConfig.create(1, H, D, D, num_slots=3), device=gpu) for _ in range(2)]
+    got = op(*parts, views[0], meta, decays).attention_outputs
+    want = op(*(x.contiguous() for x in parts), views[1], meta, decays).attention_outputs
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(views[0].state, views[1].state) and torch.isfinite(got).all()

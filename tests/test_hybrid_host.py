@@ -70,3 +70,25 @@ def test_reading_operations_refuse_a_rotation():
     with pytest.raises(NotImplementedError, match="shard-local"):
         pool = torch.zeros(1, 16, 1, 8)
         OperationRegistry.create("unified_attention", OperationMetadata()).forward_dp_local_shard(q, pool, pool, meta, 0, 1, rope=r)
+
+
+def test_the_linear_layer_takes_parts_of_every_head(monkeypatch):
+    """One projection reshaped to heads and split inside each head, with and without a batch axis; rows of a projection stay where they are."""
+    from easydel_amd import kernels
+
+    seen = []
+    monkeypatch.setattr(kernels, "decay_linear_attention", lambda q, k, v, g, state, *a, **kw: (seen.append((q, k, v)) or q.new_zeros(*q.shape[:2], v.shape[2]), state))
+    op = OperationRegistry.create("ragged_decay_linear_attention", OperationMetadata())
+    view = DecayStateCacheView.init(DecayStateCacheConfig.create(1, 2, 16, 32, num_slots=3), device="cpu")
+    i = torch.zeros(3, dtype=torch.int32)
+    meta = DecayStateMetadata(query_start_loc=i, num_seqs=i[:1], state_indices=i[:2])
+    heads = torch.arange(5 * 2 * 64.0).reshape(5, 2, 64)
+    parts = heads.split((16, 16, 32), -1)
+    for lead in ((), (1,)):
+        out = op(*(x.reshape(*lead, *x.shape) for x in parts), view, meta, torch.zeros(2)).attention_outputs
+        assert out.shape == (*lead, 5, 2, 32)
+        for got, want in zip(seen.pop(), parts):
+            assert torch.equal(got, want) and got[0].is_contiguous()
+    rows = [x.unflatten(1, (2, -1)) for x in heads.flatten(1).split((32, 32, 64), 1)]
+    op(*rows, view, meta, torch.zeros(2))
+    assert [x.data_ptr() for x in seen.pop()] == [x.data_ptr() for x in rows]
