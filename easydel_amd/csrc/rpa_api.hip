@@ -942,7 +942,7 @@ static void decay_segments(int T, int S, int Hkv, int Dk, int Dv, rpa::DecayPara
   const int64_t fill = ((int64_t)T * Hkv * slices + 2 * cus - 1) / (2 * cus);
   const int64_t len = std::max((fill + 63) / 64 * 64, std::min<int64_t>((2 * fill + 63) / 64 * 64, 256));
   p.seg_len = (int)std::min<int64_t>(len, (int64_t)1 << 30);
-  p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, std::max(p.seg_len, 256)), (int64_t)1 << 30);
+  p.whole_len = (int)std::min<int64_t>(std::max<int64_t>(2 * fill, std::max(p.seg_len, rpa::kDecayWhole)), (int64_t)1 << 30);
   p.slots = T > p.whole_len ? T / p.seg_len + 1 : 0;
   const int by_token = T / (rpa::kDecayRows + 1) + 1;
   p.first_by_seq = S <= by_token;

@@ -36,6 +36,7 @@ struct DecayParams {
 };
 
 constexpr int kDecayRows = 16;
+constexpr int kDecayWhole = 256;  // sequences of up to this many tokens are never cut (the Python layer asks for no scratch below it either)
 
 struct DecaySeq {
   int q0, q_len;

@@ -637,6 +637,9 @@ def rope_mla_page_scatter(queries_pe, keys_values, keys_pe, kv_pages, cos_sin, c
     return out, kv_pages
 
 
+_DECAY_WHOLE = 256  # kDecayWhole of rpa_decay.h: calls of up to this many tokens need no scratch
+
+
 def decay_linear_attention(query, key, value, log_decay, state, state_indices, query_start_loc, num_seqs, *, context_lens=None,
                            state_out_indices=None, scale: float | None = None, out=None):
     """Linear attention with one decay per KV head over a ragged batch; the states live in the slots of a pool.
@@ -695,7 +698,7 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
         tag = _DTYPE_TAG[dt]
         # scratch of its own for every call: the caching allocator orders its reuse by stream, and a captured graph keeps its own
         need = 0
-        if T > 256:  # nothing is cut below that
+        if T > _DECAY_WHOLE:
             with torch.cuda.device(dev):  # the size goes by the current device's compute units
                 need = lib.rpa_decay_attention_workspace_bytes(T, S, Hq, Hkv, Dk, Dv, tag)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

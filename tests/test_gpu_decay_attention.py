@@ -418,3 +418,21 @@ def test_no_tokens(gpu):
     out, state = call(d)  # no live row: outputs are zeros, states as they were
     torch.cuda.synchronize()
     assert not out.any() and torch.equal(state, want)
+
+
+def test_scratch_starts_where_the_wrapper_asks_for_it(gpu):
+    """The library cuts nothing in calls of up to as many tokens as the wrapper does not ask for; calls around that border run."""
+    from easydel_amd import _lib
+
+    lib, whole = _lib.load(), kernels._DECAY_WHOLE
+    sizes = [(S, Hkv, dk, dv) for S in (1, 7, 4000) for Hkv in (1, 2, 64) for dk, dv in ((4, 4), (128, 128), (256, 256))]
+    need = lambda T: [lib.rpa_decay_attention_workspace_bytes(T, S, Hkv, Hkv, dk, dv, 1) for S, Hkv, dk, dv in sizes]  # noqa: E731
+    for T in (1, 16, 17, 100, whole - 1, whole):
+        assert not any(need(T))
+    assert any(need(whole + 1))
+    for T in (whole - 1, whole, whole + 1, whole + 2):
+        c = make(90, [T], Hq=1, Hkv=1, Dk=64, Dv=64)
+        d = upload(c, gpu)
+        out, state = call(d)
+        torch.cuda.synchronize()
+        check(c, out, state)
