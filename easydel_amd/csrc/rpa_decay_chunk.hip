@@ -202,7 +202,7 @@ __device__ __forceinline__ void store_state(const DecayParams& p, const Segment&
 // What a chunk costs is mostly the latency of its chain (tiles, scores, barrier, products, store); sixteen waves a CU with 16
 // columns each hide it better than eight with 32 (152 against 127 us below).
 // Measured: one prompt of 16384 tokens, 32 heads of 128 x 128: sums 70 us (268 MB, 3.8 TB/s), scan 14 us, outputs 126 to 146 us (537 MB,
-// 3.7 to 4.3 TB/s).  In a round of two workgroups a CU (9400 cycles) the matrix units work for 2400 cycles, LDS for
+// 3.7 to 4.3 TB/s).  In a round of two workgroups a CU (9400 cycles) the matrix units work for 2300 cycles, LDS for
 // 2300, the vector units for 3900, one after the other more than side by side.
 
 constexpr int kChunk = 32;

@@ -649,8 +649,9 @@ def decay_linear_attention(query, key, value, log_decay, state, state_indices, q
     apart) and ``state [slots, Hkv, Dk, Dv]`` float32, one state to ``Hq / Hkv`` query heads.  Sequence ``i`` goes on from slot
     ``state_indices[i]``, or from zero where ``context_lens[i]`` says that it has no tokens before these, and leaves its
     state in ``state_out_indices[i]`` (default: the same slot); slots written must differ from each other and from those that other
-    sequences of the call read.  ``scale`` defaults to ``Dk ** -0.5``.  Returns ``(out [T, Hq,
-    Dv], state)``: the pool updated in place, rows of padded tokens zeros."""
+    sequences of the call read.  ``scale`` defaults to ``Dk ** -0.5``.  States and sums are float32; in sequences of more than 16
+    tokens bfloat16 rows aligned to 16 bytes round the scores inside a chunk, and the state where it meets a query, to bfloat16 on
+    their way to the outputs.  Returns ``(out [T, Hq, Dv], state)``: the pool updated in place, rows of padded tokens zeros."""
     lib = _lib.load()
     if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
         raise ValueError(f"query [T, Hq, Dk], key [T, Hkv, Dk] and value [T, Hkv, Dv] expected, got {list(query.shape)}, "

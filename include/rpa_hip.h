@@ -377,9 +377,14 @@ int rpa_rope_mla_page_scatter(rpa_stream_t stream, const void* queries_pe, const
  *                 state whatever its slot holds.  NULL: every sequence goes on from its slot
  *   query_start_loc device, int32 [S+1]; num_seqs device, int32 [1]
  *   out           device, [T][Hq][Dv] of `dtype`; rows of padded tokens are written as zeros
- *   workspace     device, at least rpa_decay_attention_workspace_bytes(...) bytes, 256-byte aligned (NULL if that is 0)
+ *   workspace     device, at least rpa_decay_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL if that is 0)
  * A slot outside [0, num_slots) reads as a zero state and is not written.  Sequences without tokens keep their slots as they are
- * (nothing is copied to state_out_indices either).  State and sums are float32 throughout.
+ * (nothing is copied to state_out_indices either).
+ * States, decays and sums are float32 for every dtype, and outputs are rounded once to `dtype`, but for one case: in sequences of more than
+ * 16 tokens of the call, RPA_BF16 rows aligned to 16 bytes (pointers, strides, Dk and Dv) go through bfloat16 matrix instructions, and on
+ * the way to the outputs the decayed scores among 32 neighbouring tokens and the state that meets a query are rounded to bfloat16,
+ * each by at most 2^-8 of itself (random values: outputs off by 2.3e-3 of their size instead of 1.7e-3, the rounding of the
+ * result).  Such an output depends on where a scheduler cuts a prompt by as much; the states do not.
  * A value that is not finite reaches its own and later tokens of its sequence only.
  * Limits: Dk, Dv multiples of 4, at most 256; Hq a multiple of Hkv; S at most 65000, and (2 S + T / 64) * Hkv * ceil(Dv / 128) below
  * 2^23 (workgroups of a launch).
