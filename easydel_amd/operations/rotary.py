@@ -36,9 +36,12 @@ class Rotary:
 def token_rows(t: torch.Tensor) -> torch.Tensor:
     """``t [T, ...]`` with token rows that a kernel reads in place: contiguous each, however far apart.  Rows of a projection are; parts of
     every head (and one row for all tokens) are copied."""
-    if t.is_contiguous() or t.shape[0] == 0:
+    shape, apart = t.shape, t.stride()
+    if len(shape) == 3 and apart[2] == 1 and apart[1] == shape[2] and apart[0] >= shape[1] * shape[2]:  # the common case, in few steps
         return t
-    return t if t[0].is_contiguous() and (t.shape[0] == 1 or t.stride(0) >= t[0].numel()) else t.contiguous()
+    if t.is_contiguous() or shape[0] == 0:
+        return t
+    return t if t[0].is_contiguous() and (shape[0] == 1 or apart[0] >= t[0].numel()) else t.contiguous()
 
 
 def rotation_operands(result: torch.dtype, *operands: torch.Tensor) -> list[torch.Tensor]:

@@ -130,3 +130,15 @@ def test_narrowing_is_told_with_rope_as_without(latent, v3, caplog):
         caplog.clear()
         v3(q, key, value, kvdtype, scaled)
         assert ("lower-precision KV cache dtype" in caplog.text) == told
+
+
+def test_token_rows_are_copied_only_where_they_must_be():
+    from easydel_amd.operations.rotary import token_rows
+
+    x = torch.arange(6 * 5 * 8.0).reshape(6, 5, 8)
+    for t, stays in ((x, True), (x[:, 1:3], True), (x[::2], True), (x[:, 2], True), (x[:1, 1:], True), (x[:, :, :1], False), (x[:0, :, :4], True),
+                     (x[:, :, :4], False), (x[:, ::2], False), (x.transpose(0, 1), False), (x[:1].expand(6, 5, 8), False), (x[:, :1, :4], True), (x[:1, :, :4], False),
+                     (x[:, 0, ::2], False), (x[:, 0, :0], True)):
+        got = token_rows(t)
+        assert torch.equal(got, t) and (got is t) == stays, (t.shape, t.stride())
+        assert got.shape[0] == 0 or got[0].is_contiguous()
